@@ -241,7 +241,7 @@ def prepare(case, seed):
     if own:
         from flash_attn_with_score_amd import kv_cache
 
-        st["cache"] = kv_cache.KVCache(**parts, dtype=dtype)
+        st["cache"] = kv_cache.KVCache(**parts, dtype=dtype, bits=bits)
     else:
         st.update(parts)
     if op == "attend":
