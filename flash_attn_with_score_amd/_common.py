@@ -137,12 +137,19 @@ def workspace(variant: int, args, split: int, device,
     if type(args) is not bytes:  # an AttnArgs
         args = bytes(args)
     nbytes = _native.fast("fas_workspace_bytes")(variant, args, int(split))
-    if nbytes == _SIZE_MAX:
-        raise RuntimeError(
-            f"fas_workspace_bytes: {_native.last_error(_native.load()) or 'invalid request'}")
-    if nbytes == 0 or (limit is not None and nbytes > limit):
+    if limit is not None and limit < nbytes != _SIZE_MAX:
         return 0, nbytes, None
+    ptr, buf = allocate_workspace("fas_workspace_bytes", nbytes, device)
+    return ptr, nbytes, buf
+
+
+def allocate_workspace(fn_name: str, nbytes: int, device) -> tuple[int, torch.Tensor | None]:
+    """(256-byte aligned pointer, tensor) of the nbytes that the C function fn_name
+    asked for, (0, None) for none; raises if it refused the request."""
+    if nbytes == _SIZE_MAX:
+        raise RuntimeError(f"{fn_name}: {_native.last_error(_native.load()) or 'invalid request'}")
+    if nbytes == 0:
+        return 0, None
     buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
     ptr = buf.data_ptr()
-    ptr += (-ptr) % 256
-    return ptr, nbytes, buf
+    return ptr + (-ptr) % 256, buf

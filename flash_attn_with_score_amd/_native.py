@@ -154,7 +154,88 @@ _SIGNATURES = {
                        *_WS, ctypes.c_void_p]),
 }
 
-EXPORTED_SYMBOLS = tuple(_SIGNATURES)
+
+
+class KVCacheArgs(ctypes.Structure):
+    """Mirror of struct fas_kv_cache (include/fas.h)."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("capacity", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("k_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("k_codes_stride", _I64x3),
+        ("k_scales_stride", _I64x3),
+        ("v_codes_stride", _I64x3),
+        ("v_scales_stride", _I64x3),
+    ]
+
+
+class KVQueryArgs(ctypes.Structure):
+    """Mirror of struct fas_kv_query (include/fas.h)."""
+
+    _fields_ = [
+        ("heads_q", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_stride", _I64x4),
+        ("out_stride", _I64x4),
+        ("lengths", ctypes.c_void_p),
+        ("lengths_all", ctypes.c_int64),
+        ("counts", ctypes.c_void_p),
+        ("window", ctypes.c_int64),
+        ("sinks", ctypes.c_int64),
+        ("sm_scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+# Both as one packed record each (no padding in the C structs).
+_KV_CACHE_PACK = struct.Struct("<ii4q4Q12q")
+_KV_QUERY_PACK = struct.Struct("<2q2Q8qQqQ2qfi")
+assert _KV_CACHE_PACK.size == ctypes.sizeof(KVCacheArgs)
+assert _KV_QUERY_PACK.size == ctypes.sizeof(KVQueryArgs)
+
+
+def pack_kv_cache(k_codes, k_scales, v_codes, v_scales, dtype, bits: int, head_dim: int) -> bytes:
+    arrays = (k_codes, k_scales, v_codes, v_scales)
+    return _KV_CACHE_PACK.pack(
+        DTYPE_CODES[dtype], bits, *k_codes.shape[:3], head_dim,
+        *(t.data_ptr() for t in arrays), *(n for t in arrays for n in t.stride()[:3]))
+
+
+def pack_kv_query(q, out, lengths, lengths_all: int, counts, window: int, sinks: int,
+                  sm_scale: float) -> bytes:
+    """lengths, counts: device tensors or None."""
+    return _KV_QUERY_PACK.pack(
+        q.shape[1], q.shape[2], q.data_ptr(), out.data_ptr(), *q.stride(), *out.stride(),
+        0 if lengths is None else lengths.data_ptr(), lengths_all,
+        0 if counts is None else counts.data_ptr(), window, sinks, sm_scale, 0)
+
+
+# Entry points with argument records of their own.
+_CACHE, _QUERY = _P(KVCacheArgs), _P(KVQueryArgs)
+_CACHE_SIGNATURES = {
+    "fas_kv_cache_append": (
+        ctypes.c_int, [_CACHE, ctypes.c_void_p, _I64x4, ctypes.c_void_p, _I64x4, ctypes.c_int64,
+                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "fas_kv_cache_read": (
+        ctypes.c_int, [_CACHE, ctypes.c_void_p, _I64x4, ctypes.c_void_p, _I64x4, ctypes.c_int64,
+                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "fas_attention_kv_cache_workspace": (ctypes.c_size_t, [_CACHE, _QUERY]),
+    "fas_attention_kv_cache": (
+        ctypes.c_int, [_CACHE, _QUERY, ctypes.c_void_p, _I64x3, *_WS, ctypes.c_void_p]),
+}
+_ALL_SIGNATURES = {**_SIGNATURES, **_CACHE_SIGNATURES}
+
+EXPORTED_SYMBOLS = tuple(_ALL_SIGNATURES)
 
 
 def library_path() -> Path:
@@ -184,7 +265,7 @@ def load() -> ctypes.CDLL:
                 "`python -c 'import __graft_entry__ as g; g.build()'` or "
                 "`python flash_attn_with_score_amd/csrc/build.py`")
         lib = ctypes.CDLL(str(path))
-        for name, (restype, argtypes) in _SIGNATURES.items():
+        for name, (restype, argtypes) in _ALL_SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -194,8 +275,8 @@ def load() -> ctypes.CDLL:
         # The same entry points taking their records as bytes: no ctypes
         # structure or array is built per call.
         records = ctypes.CDLL(str(path))
-        swap = {_P(AttnArgs): ctypes.c_char_p, _I64x4: ctypes.c_char_p, _I64x3: ctypes.c_char_p}
-        for name, (restype, argtypes) in _SIGNATURES.items():
+        swap = {t: ctypes.c_char_p for t in (_P(AttnArgs), _CACHE, _QUERY, _I64x4, _I64x3)}
+        for name, (restype, argtypes) in _ALL_SIGNATURES.items():
             fn = getattr(records, name)
             fn.restype = restype
             fn.argtypes = [swap.get(t, t) for t in argtypes]

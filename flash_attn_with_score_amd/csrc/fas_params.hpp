@@ -296,3 +296,58 @@ struct ScoresParams {
 };
 
 }  // namespace fas
+
+namespace fas {
+
+// Rows of the quantised KV cache in or out (fas_cache.hpp).  Strides of the
+// rows are in elements, those of codes and scales in bytes.
+struct CacheSide {
+  uint16_t* rows;  // (B, H, M, D)
+  uint8_t* codes;  // (B, H, capacity, D * bits / 8)
+  uint8_t* scales; // (B, H, capacity, max(1, D / 32))
+  int64_t sr0, sr1, sr2;
+  int64_t sc0, sc1, sc2;
+  int64_t ss0, ss1, ss2;
+};
+struct CacheParams {
+  CacheSide side[2];       // keys, values
+  const int32_t* start;    // (B,) cache row of each sequence's row 0, or null: start_all
+  const int32_t* counts;   // append: (B,) rows written per sequence, or null: M
+  int start_all;
+  int B, H, M, capacity;
+  int chunks;              // workgroups per tensor, batch entry and head
+};
+
+// Most workgroups that share a row's keys (cache_merge_kernel holds one part a
+// thread).
+constexpr int kCacheMaxSplits = 256;
+
+// Attention over the quantised cache (fas_cache_attn.hpp).
+struct CacheAttnParams {
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;              // optional (B, H, M)
+  const uint8_t *kc, *ks, *vc, *vs;
+  int64_t sq0, sq1, sq2;
+  int64_t so0, so1, so2;
+  int64_t sl0, sl1, sl2;
+  int64_t skc0, skc1, skc2, sks0, sks1, sks2;
+  int64_t svc0, svc1, svc2, svs0, svs1, svs2;
+  const int32_t* lengths;  // (B,) or null: lengths_all
+  const int32_t* counts;   // (B,) or null: M
+  int lengths_all;
+  int B, H, Hk, G, M, capacity;
+  int window, sinks;       // window at most kCacheNoWindow
+  int nrb;                 // cache_rows_kernel: blocks of 128 virtual rows
+  int nsplit;              // workgroups per row block, at most kCacheMaxSplits
+  int min_tiles;           // least key tiles of a workgroup
+  int Rpad;                // virtual rows, padded to whole blocks
+  float* part_o;           // (B * Hk, nsplit, Rpad, D): unnormalised O
+  float* part_ml;          // (B * Hk, nsplit, Rpad, 2): base-2 exponent offset, sum of weights
+  float qk_scale;          // |sm_scale| * log2(e)
+  uint32_t qneg;           // 0x80008000 to negate q (negative sm_scale), else 0
+};
+// Window of a call without one; pos - window stays inside 32 bits.
+constexpr int kCacheNoWindow = 1 << 30;
+
+}  // namespace fas

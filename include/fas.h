@@ -281,6 +281,86 @@ int fas_attention_backward(const fas_attn_args* a, const void* dout,
                            const int64_t dv_stride[4], void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---- Quantised KV cache.  No counterpart in the reference. ----
+ *
+ * The keys and values of a batch of sequences, (batch, heads, capacity,
+ * head_dim), held as codes of 4 or 8 bits with a power-of-two scale per block
+ * of 32 channels (16 for head_dim 16).  bits = 4: e2m1 codes (0, .5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives), channel 2i in the low half of byte i; bits = 8:
+ * e4m3 codes (largest 448).  A scale byte x stands for 2^(x - 127); 255 makes
+ * every value of the block NaN.  Each array's rows are contiguous (head_dim *
+ * bits / 8 bytes of codes, max(1, head_dim / 32) of scales) and aligned to
+ * their size, up to 16 bytes; the strides are in bytes, (batch, head, token).
+ *
+ * Per-sequence numbers (start, lengths, counts) are int32 device arrays of
+ * `batch` elements, read when the kernels run, so that a captured call follows
+ * them; what they say is bounded on the device.  A NULL array means the same
+ * number, passed beside it and checked on the host, for every sequence. */
+typedef struct fas_kv_cache {
+  int32_t dtype; /* fas_dtype of the values */
+  int32_t bits;  /* 4 or 8 */
+  int64_t batch, heads, capacity, head_dim;
+  void* k_codes;
+  void* k_scales;
+  void* v_codes;
+  void* v_scales;
+  int64_t k_codes_stride[3];
+  int64_t k_scales_stride[3];
+  int64_t v_codes_stride[3];
+  int64_t v_scales_stride[3];
+} fas_kv_cache;
+
+/* Quantises rows of k and v (batch, heads, tokens, head_dim) into the cache:
+ * row i of sequence b becomes cache row start[b] + i, for i < counts[b] (all of
+ * them with counts NULL).  Rows that would fall outside [0, capacity) are not
+ * written, and no other row of the cache changes.  A block's scale is the least
+ * power of two s (at least 2^-126) with amax <= C s, C = 6 or 448, but no
+ * larger than keeps C s finite in the value type (2^13 and 2^7 for fp16, 2^125
+ * and 2^119 for bf16); values round to the nearest code, ties to even, those
+ * past C s to C s.  A block with an infinity or NaN reads as NaN. */
+int fas_kv_cache_append(const fas_kv_cache* cache, const void* k, const int64_t k_stride[4],
+                        const void* v, const int64_t v_stride[4], int64_t tokens,
+                        const int32_t* start, int64_t start_all, const int32_t* counts,
+                        void* stream);
+
+/* Cache rows start[b] .. start[b] + tokens - 1 as values in the cache's type
+ * (exact), into k and v (batch, heads, tokens, head_dim); rows outside
+ * [0, capacity) read as zeros. */
+int fas_kv_cache_read(const fas_kv_cache* cache, void* k, const int64_t k_stride[4], void* v,
+                      const int64_t v_stride[4], int64_t tokens, const int32_t* start,
+                      int64_t start_all, void* stream);
+
+/* The queries of fas_attention_kv_cache: q and out (batch, heads_q, tokens,
+ * head_dim) in the cache's value type, strides in elements. */
+typedef struct fas_kv_query {
+  int64_t heads_q, tokens;
+  const void* q;
+  void* out;
+  int64_t q_stride[4];
+  int64_t out_stride[4];
+  const int32_t* lengths; /* keys each sequence holds, or NULL: lengths_all */
+  int64_t lengths_all;
+  const int32_t* counts;  /* query rows of each sequence, or NULL: tokens */
+  int64_t window;         /* keys a row sees up to its own; 0: all of them */
+  int64_t sinks;          /* first keys that stay visible behind the window */
+  float sm_scale;
+  int32_t reserved;
+} fas_kv_query;
+
+/* Attention of each sequence's last counts[b] tokens over its lengths[b] cached
+ * keys (its own among them): row i is at position lengths[b] - counts[b] + i
+ * and sees key j iff j <= position and (j > position - window or j < sinks).
+ * Rows past counts[b], and rows that see no key, give out = 0 and lse = -inf.
+ * lengths are bounded to [0, capacity] and counts to [0, tokens].  lse
+ * (batch, heads_q, tokens) fp32 takes the natural-log normalizer; NULL: not
+ * wanted.  Cache rows past a sequence's length do not influence it, whatever
+ * they hold.  The workspace is fas_attention_kv_cache_workspace(cache, query)
+ * bytes, 256-byte aligned ((size_t)-1: invalid request). */
+size_t fas_attention_kv_cache_workspace(const fas_kv_cache* cache, const fas_kv_query* query);
+int fas_attention_kv_cache(const fas_kv_cache* cache, const fas_kv_query* query, float* lse,
+                           const int64_t lse_stride[3], void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif
