@@ -107,7 +107,7 @@ def _raw_stream(index: int) -> int:
 
 # torch's current stream of a device as a raw handle without building a
 # Stream object (the call costs ~0.3 us instead of several).
-_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -117,10 +117,10 @@ def call(fn_name: str, q: torch.Tensor, *args) -> None:
     fn = _native.fast(fn_name)
     index = q.device.index
     if index == _current_device():
-        rc = fn(*args, _current_raw_stream(index))
+        rc = fn(*args, current_raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _current_raw_stream(index))
+            rc = fn(*args, current_raw_stream(index))
     if rc:
         _native.check(_native.load(), rc, fn_name)
 

@@ -220,7 +220,19 @@ def pack_kv_query(q, out, lengths, lengths_all: int, counts, window: int, sinks:
         0 if counts is None else counts.data_ptr(), window, sinks, sm_scale, 0)
 
 
-# Entry points with argument records of their own.
+# Attention with a sliding window and sinks.
+_WINDOW_SIGNATURES = {
+    "fas_attention_window_workspace": (
+        ctypes.c_size_t, [_P(AttnArgs), ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "fas_attention_window": (
+        ctypes.c_int, [_P(AttnArgs), ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, _I64x3, *_WS,
+                       ctypes.c_void_p]),
+    "fas_attention_window_backward": (
+        ctypes.c_int, [_P(AttnArgs), ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, _I64x4,
+                       ctypes.c_void_p, _I64x3, ctypes.c_void_p, _I64x4, ctypes.c_void_p, _I64x4,
+                       ctypes.c_void_p, _I64x4, *_WS, ctypes.c_void_p]),
+}
+# The quantised KV cache: argument records of its own.
 _CACHE, _QUERY = _P(KVCacheArgs), _P(KVQueryArgs)
 _CACHE_SIGNATURES = {
     "fas_kv_cache_append": (
@@ -233,7 +245,7 @@ _CACHE_SIGNATURES = {
     "fas_attention_kv_cache": (
         ctypes.c_int, [_CACHE, _QUERY, ctypes.c_void_p, _I64x3, *_WS, ctypes.c_void_p]),
 }
-_ALL_SIGNATURES = {**_SIGNATURES, **_CACHE_SIGNATURES}
+_ALL_SIGNATURES = {**_SIGNATURES, **_WINDOW_SIGNATURES, **_CACHE_SIGNATURES}
 
 EXPORTED_SYMBOLS = tuple(_ALL_SIGNATURES)
 

@@ -53,38 +53,19 @@ int fas::device_cu_count() {
   return cache[(size_t)dev];
 }
 
-namespace {
-
-using fas::align256;
-using fas::check_tensor;
-using fas::device_cu_count;
-using fas::fail;
-using fas::hip_status;
-using fas::kMaxOuterStride;
-using fas::kMaxSliceBytes;
-using fas::qk_scale_of;
-using fas::slice_bytes;
-using fas::strides_out_of_range;
-
-struct Problem {
-  int B, H, Hk, G, M, N, D, dtype, causal;
-  bool dropout;  // dropout_p > 0
-  bool keep;     // dropout with a caller keep-bit buffer (fas_attn_args.keep_bits)
-  float sm_scale;
-  int pack;  // query heads per forward workgroup (GQA packing): G, or 1
-};
+namespace fas {
 
 // Bytes a 16-bit (B, H, L, D) tensor spans over `heads` consecutive heads of
 // one batch entry, including the tile overhang the kernels may address past
 // the last row.
-int64_t head_span_bytes(const int64_t* st, int64_t heads, int64_t rows) {
+static int64_t head_span_bytes(const int64_t* st, int64_t heads, int64_t rows) {
   return ((heads - 1) * st[1] + (rows + 512) * st[2]) * 2;
 }
 
 // GQA packing: a forward workgroup serves all G query heads of a KV head
 // when the G heads of q and out can be addressed with 32-bit offsets from
 // the first (the kernels mark invalid rows with offset 2^31).
-int choose_pack(const fas_attn_args* a, int G, int M) {
+static int choose_pack(const fas_attn_args* a, int G, int M) {
   // Launches with dropout keep one head per workgroup (no packed dropout
   // instances are built).
   if (G <= 1 || a->dropout_p > 0.f) return 1;
@@ -157,6 +138,25 @@ int check_args(const char* fn, const fas_attn_args* a, Problem* pr) {
   }
   return FAS_OK;
 }
+
+}  // namespace fas
+
+namespace {
+
+using fas::align256;
+using fas::check_args;
+using fas::check_shape;
+using fas::check_tensor;
+using fas::device_cu_count;
+using fas::fail;
+using fas::hip_status;
+using fas::kCus;
+using fas::kMaxOuterStride;
+using fas::kMaxSliceBytes;
+using fas::Problem;
+using fas::qk_scale_of;
+using fas::slice_bytes;
+using fas::strides_out_of_range;
 
 // Dropout threshold: the largest y in [0, 2^31 - 1] whose uniform
 // float(y) * 4.6566127342e-10 (Triton's uint_to_uniform_float, fp32) is
@@ -297,7 +297,6 @@ struct ColPlan {
   int fold = 1, nsplit = 1;
   int64_t nunits = 0, ngroups = 0;
 };
-constexpr int64_t kCus = 256;  // MI355X compute units
 // split_rows: false deals whole heads only (less room for partials).
 ColPlan col_plan(const Problem& pr, bool buffered, int64_t ncols, int64_t row_lo,
                  bool split_rows) {

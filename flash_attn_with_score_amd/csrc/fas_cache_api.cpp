@@ -16,6 +16,7 @@
 #include "fas_check.hpp"
 #include "fas_launch.hpp"
 #include "fas_params.hpp"
+#include "fas_rows_plan.hpp"
 
 namespace {
 
@@ -123,12 +124,6 @@ int move_rows(const char* fn, bool append, const fas_kv_cache* c, const void* k,
                                : fas::launch_cache_read(p, c->dtype, d, c->bits, s));
 }
 
-// How an attention call is dealt to workgroups.
-struct AttnPlan {
-  int64_t nrb, nsplit, min_tiles, rpad;
-  size_t part_o, part_ml, total;  // workspace: offsets and bytes
-};
-
 int check_attn(const char* fn, const fas_kv_cache* c, const fas_kv_query* a) {
   int rc;
   if ((rc = check_cache_shape(fn, c))) return rc;
@@ -150,34 +145,11 @@ int check_attn(const char* fn, const fas_kv_cache* c, const fas_kv_query* a) {
   return FAS_OK;
 }
 
-// Workgroups of one round (two a CU), and the fewest keys worth a workgroup of
-// their own.
-AttnPlan attn_plan(const fas_kv_cache* c, const fas_kv_query* a) {
-  AttnPlan w{};
+fas::RowsSplit attn_split(const fas_kv_cache* c, const fas_kv_query* a) {
   const int64_t rows = a->heads_q / c->heads * a->tokens;
-  const bool few = rows <= fas::kCacheFewRows;
-  const int64_t bm = few ? fas::kCacheFewRows : fas::kCacheBlockRows;
-  const int64_t bn = few ? fas::kCacheFewKeys : fas::kCacheBlockKeys;
-  w.nrb = (rows + bm - 1) / bm;
-  w.rpad = w.nrb * bm;
-  // Key tiles that a row block can need, whatever the sequences' lengths.
-  int64_t keys = a->lengths == nullptr ? a->lengths_all : c->capacity;
-  if (a->window > 0)
-    keys = std::min(keys, std::min(a->window, keys) + std::min(a->sinks, keys) +
-                              std::min(a->tokens, bm) + 2 * bn);
-  const int64_t tiles = (keys + bn - 1) / bn;
-  w.min_tiles = few ? 16 : 8;
-  const int64_t blocks = c->batch * c->heads * w.nrb, slots = 2 * (int64_t)fas::device_cu_count();
-  w.nsplit = 1;
-  if (blocks > 0 && blocks < slots)
-    w.nsplit = std::max<int64_t>(1, std::min({(slots + blocks - 1) / blocks, tiles / w.min_tiles,
-                                              (int64_t)fas::kCacheMaxSplits}));
-  if (w.nsplit > 1) {
-    const size_t n = (size_t)(c->batch * c->heads * w.nsplit * w.rpad);
-    w.part_ml = fas::align256(n * (size_t)c->head_dim * 4);
-    w.total = w.part_ml + fas::align256(n * 8);
-  }
-  return w;
+  return fas::rows_split(c->batch * c->heads, rows, a->tokens,
+                         a->lengths == nullptr ? a->lengths_all : c->capacity, a->window, a->sinks,
+                         c->head_dim, rows <= fas::kCacheFewRows);
 }
 
 }  // namespace
@@ -200,7 +172,7 @@ int fas_kv_cache_read(const fas_kv_cache* c, void* k, const int64_t kst[4], void
 
 size_t fas_attention_kv_cache_workspace(const fas_kv_cache* c, const fas_kv_query* a) {
   if (check_attn("fas_attention_kv_cache_workspace", c, a)) return (size_t)-1;
-  return attn_plan(c, a).total;
+  return attn_split(c, a).total;
 }
 
 int fas_attention_kv_cache(const fas_kv_cache* c, const fas_kv_query* a, float* lse,
@@ -219,28 +191,26 @@ int fas_attention_kv_cache(const fas_kv_cache* c, const fas_kv_query* a, float* 
     if (fas::strides_out_of_range(lst, 3))
       return fail(FAS_ERR_INVALID, fn, "lse strides must lie in [0, 2^46)");
   }
-  const AttnPlan w = attn_plan(c, a);
-  if (w.total > 0 && (ws == nullptr || ws_bytes < w.total || reinterpret_cast<uintptr_t>(ws) % 256))
-    return fail(FAS_ERR_WORKSPACE, fn, "needs %zu bytes of workspace aligned to 256, got %zu at %p",
-                w.total, ws_bytes, ws);
+  const fas::RowsSplit w = attn_split(c, a);
+  if ((rc = fas::check_rows_workspace(fn, w.total, ws, ws_bytes))) return rc;
   if (c->batch * c->heads * w.nrb * w.nsplit > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more row blocks than one launch takes");
-  fas::CacheAttnParams p{};
+  fas::RowsParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
   p.o = static_cast<uint16_t*>(a->out);
   p.lse = lse;
-  p.kc = static_cast<const uint8_t*>(c->k_codes);
+  p.k = static_cast<const uint8_t*>(c->k_codes);
   p.ks = static_cast<const uint8_t*>(c->k_scales);
-  p.vc = static_cast<const uint8_t*>(c->v_codes);
+  p.v = static_cast<const uint8_t*>(c->v_codes);
   p.vs = static_cast<const uint8_t*>(c->v_scales);
   p.sq0 = a->q_stride[0]; p.sq1 = a->q_stride[1]; p.sq2 = a->q_stride[2];
   p.so0 = a->out_stride[0]; p.so1 = a->out_stride[1]; p.so2 = a->out_stride[2];
   if (lse != nullptr) {
     p.sl0 = lst[0]; p.sl1 = lst[1]; p.sl2 = lst[2];
   }
-  p.skc0 = c->k_codes_stride[0]; p.skc1 = c->k_codes_stride[1]; p.skc2 = c->k_codes_stride[2];
+  p.sk0 = c->k_codes_stride[0]; p.sk1 = c->k_codes_stride[1]; p.sk2 = c->k_codes_stride[2];
   p.sks0 = c->k_scales_stride[0]; p.sks1 = c->k_scales_stride[1]; p.sks2 = c->k_scales_stride[2];
-  p.svc0 = c->v_codes_stride[0]; p.svc1 = c->v_codes_stride[1]; p.svc2 = c->v_codes_stride[2];
+  p.sv0 = c->v_codes_stride[0]; p.sv1 = c->v_codes_stride[1]; p.sv2 = c->v_codes_stride[2];
   p.svs0 = c->v_scales_stride[0]; p.svs1 = c->v_scales_stride[1]; p.svs2 = c->v_scales_stride[2];
   p.lengths = a->lengths;
   p.lengths_all = a->lengths == nullptr ? (int)a->lengths_all : 0;
@@ -251,17 +221,10 @@ int fas_attention_kv_cache(const fas_kv_cache* c, const fas_kv_query* a, float* 
   p.G = p.H / p.Hk;
   p.M = (int)a->tokens;
   p.capacity = (int)c->capacity;
-  p.window = a->window == 0 ? fas::kCacheNoWindow
-                            : (int)std::min<int64_t>(a->window, fas::kCacheNoWindow);
-  p.sinks = (int)std::min<int64_t>(a->sinks, fas::kCacheNoWindow);
-  p.nrb = (int)w.nrb;
-  p.nsplit = (int)w.nsplit;
-  p.min_tiles = (int)w.min_tiles;
-  p.Rpad = (int)w.rpad;
-  if (w.nsplit > 1) {
-    p.part_o = static_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + w.part_ml);
-  }
+  p.window = a->window == 0 ? fas::kNoWindow
+                            : (int)std::min<int64_t>(a->window, fas::kNoWindow);
+  p.sinks = (int)std::min<int64_t>(a->sinks, fas::kNoWindow);
+  fas::apply_rows_split(p, w, ws);
   p.qk_scale = fas::qk_scale_of(a->sm_scale);
   p.qneg = a->sm_scale < 0.f ? 0x80008000u : 0u;
   return hip_status(fn, fas::launch_cache_attn(p, c->dtype, (int)c->head_dim, c->bits,

@@ -1,12 +1,5 @@
-// gfx950 attention over the quantised KV cache (fas_cache.hpp: its form).
-//
-// Sequence b holds len = lengths[b] keys; its cnt = counts[b] query rows are its
-// last tokens, row i at position len - cnt + i.  A row at position pos sees key
-// j iff 0 <= j <= pos and (j > pos - window or j < sinks).  Rows past cnt, and
-// rows that see no key, give O = 0 and L = -inf.
-//
-// The G query heads of a KV head read the same keys, so a workgroup takes
-// their rows together: virtual row v = i * G + j is row i of head h0 + j.
+// gfx950 attention over the quantised KV cache (fas_cache.hpp: its form;
+// fas_rows.hpp: which keys a row sees, and what is shared with dense keys).
 //
 //   cache_few_kernel    at most 32 virtual rows (decoding).  Bound by the
 //                       cache's bytes, so nothing is shared between the waves:
@@ -18,16 +11,9 @@
 //                       loaded in the same order); V codes become rows of a
 //                       small LDS tile of the wave's, which the transposing
 //                       read turns into the A operand of O^T += V^T P^T.
-//   cache_rows_kernel   more rows (a chunk of a prompt): 128 virtual rows, four
-//                       waves of 32.  Bound by the products, so tiles of 64
-//                       keys are converted once and shared through LDS: the
+//   rows_kernel         more rows (a chunk of a prompt), with CacheSource: the
 //                       codes of the next tile are fetched before the products
-//                       of the current one and converted after them.
-//   cache_merge_kernel  adds up the parts of rows whose keys were dealt to
-//                       several workgroups.
-//
-// Tiles are dealt by the length the device sees, not by the capacity the host
-// knows: every sequence spreads its own tiles evenly over its workgroups.
+//                       of the current one and converted into LDS after them.
 //
 // Keys past len are never taken as values: their row index is clamped to the
 // last key and their weight is 0.  A weight of 0 would still turn a NaN value
@@ -36,205 +22,9 @@
 // zeros, and the rows that see such a block are set to NaN afterwards.
 #pragma once
 #include "fas_cache.hpp"
+#include "fas_rows.hpp"
 
 namespace fas {
-
-// Tiles of BN keys that a block of virtual rows [row0, row0 + BM) reads:
-// the first `sink_tiles` tiles of the cache, then `tiles - sink_tiles` tiles
-// from tile `win` on, dealt to `used` workgroups in runs of `per`.
-struct CachePlan {
-  int len, cnt, pos0;  // keys, query rows, position of row 0
-  int lo, hi;          // least and greatest position of the block's live rows (hi < lo: none)
-  int sink_tiles, win, tiles, per, used;
-  __device__ __forceinline__ int tile(int i) const {
-    return i < sink_tiles ? i : i - sink_tiles + win;
-  }
-};
-template <int BM, int BN>
-__device__ __forceinline__ CachePlan cache_plan(const CacheAttnParams& p, int b, int rb) {
-  CachePlan c;
-  c.len = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.capacity) : p.lengths_all;
-  c.cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.M) : p.M;
-  c.pos0 = c.len - c.cnt;
-  const int i0 = rb * BM / p.G, i1 = min(c.cnt, (rb * BM + BM - 1) / p.G + 1);  // rows [i0, i1)
-  c.lo = c.pos0 + i0;
-  c.hi = i1 > i0 ? c.pos0 + i1 - 1 : c.lo - 1;
-  c.sink_tiles = c.win = c.tiles = 0;
-  if (c.hi >= max(c.lo, 0)) {
-    c.win = max(0, max(c.lo, 0) - p.window + 1) / BN;
-    c.sink_tiles = min(c.win, (min(p.sinks, c.hi + 1) + BN - 1) / BN);
-    c.tiles = c.sink_tiles + (c.hi + BN) / BN - c.win;
-  }
-  c.per = max(p.min_tiles, (c.tiles + p.nsplit - 1) / p.nsplit);
-  if (BM == 32) c.per = (c.per + 3) & ~3;  // cache_few_kernel's four waves take turns
-  c.used = max(1, (c.tiles + c.per - 1) / c.per);
-  return c;
-}
-
-// Whether every live row of the block sees all keys [k0, k0 + n).
-__device__ __forceinline__ bool cache_full(const CacheAttnParams& p, const CachePlan& c, int k0,
-                                           int n) {
-  return k0 + n - 1 <= c.lo && (k0 > c.hi - p.window || k0 + n <= p.sinks);
-}
-__device__ __forceinline__ bool cache_sees(const CacheAttnParams& p, int pos, int key) {
-  return key <= pos && (key > pos - p.window || key < p.sinks);
-}
-
-// Online softmax of one row a lane pair (lanes c and c + 32) over tiles of
-// 32 * NB keys; register r of s[kb] is key 32 kb + acc_row(r, g).
-template <class E, int D, int NB>
-struct CacheRows {
-  static constexpr int DB = (D + 31) / 32;
-  float m = neg_inf();  // exponent offset (a score), at most 2^8 below the row's maximum
-  float l = 0.f;        // this lane's share of the weights' sum
-  f32x16 o[DB];
-  __device__ __forceinline__ CacheRows() {
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
-  }
-  // Weights 2^(qk (s - m)) as B operands of O^T += V^T P^T; their sum (of
-  // this lane's keys) is kept in fp32.  They are rounded to the cache's type
-  // for the product alone.
-  __device__ __forceinline__ float weights(const f32x16 (&s)[NB], float qk, u32x4 (&pb)[2 * NB]) {
-    const float nb = (m == neg_inf() ? 0.f : m) * qk;
-    float lt = 0.f;
-#pragma unroll
-    for (int cs = 0; cs < 2 * NB; ++cs) {
-      float pv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pv[e] = exp2f_fast(fmaf(s[cs >> 1][8 * (cs & 1) + e], qk, -nb));
-        lt += pv[e];
-      }
-      pb[cs] = u32x4{E::pack(pv[0], pv[1]), E::pack(pv[2], pv[3]), E::pack(pv[4], pv[5]),
-                     E::pack(pv[6], pv[7])};
-    }
-    return lt;
-  }
-  // The weights are formed with the offset as it is; only where a lane's sum
-  // passes 2^14 (or is NaN), or a row has no offset yet, does the wave raise
-  // the offsets and form them again.  Every weight stays in fp16's range.
-  __device__ __forceinline__ void tile(const f32x16 (&s)[NB], float qk, u32x4 (&pb)[2 * NB]) {
-    float lt = weights(s, qk, pb);
-    const bool redo = !(lt <= 16384.f) || m == neg_inf();
-    if (__builtin_amdgcn_ballot_w64(redo) != 0) {
-      float mx = neg_inf();
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-      mx = xor32_max(mx);
-      if (mx > m && (m == neg_inf() || (mx - m) * qk > 8.f)) {
-        const float a = m == neg_inf() ? 0.f : exp2f_fast((m - mx) * qk);
-        l *= a;
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] *= a;
-        m = mx;
-      }
-      lt = weights(s, qk, pb);
-    }
-    l += lt;
-  }
-  // Adds another wave's rows (the same lanes hold the same rows).
-  __device__ __forceinline__ void save(float* a, int lane) const {
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) a[(16 * db + r) * 64 + lane] = o[db][r];
-    a[16 * DB * 64 + lane] = m;
-    a[(16 * DB + 1) * 64 + lane] = l;
-  }
-  __device__ __forceinline__ void add(const float* a, int lane, float qk) {
-    const float mo = a[16 * DB * 64 + lane], lo = a[(16 * DB + 1) * 64 + lane];
-    const float mn = fmaxf(m, mo);
-    const float a0 = m == neg_inf() ? 0.f : exp2f_fast((m - mn) * qk);
-    const float a1 = mo == neg_inf() ? 0.f : exp2f_fast((mo - mn) * qk);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] = o[db][r] * a0 + a[(16 * db + r) * 64 + lane] * a1;
-    l = l * a0 + lo * a1;
-    m = mn;
-  }
-  static constexpr int kSaved = (16 * DB + 2) * 64;  // floats
-};
-
-// NaN blocks: bit `group` of flag(row) says that the V block of tile row `row`
-// reads as NaN; rows that see the key are set to NaN there.
-template <class E, int D, int NB, class F>
-__device__ __forceinline__ void cache_set_nan(CacheRows<E, D, NB>& a, const CacheAttnParams& p,
-                                              int pos, int k0, F&& flag) {
-  for (int row = 0; row < 32 * NB; ++row) {
-    const uint32_t f = flag(row);
-    const bool sees = cache_sees(p, pos, k0 + row);
-#pragma unroll
-    for (int db = 0; db < CacheRows<E, D, NB>::DB; ++db)
-      if ((f >> db) & 1u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) a.o[db][r] = sees ? __builtin_nanf("") : a.o[db][r];
-  }
-}
-
-// O (and L) of virtual row v, or, with several workgroups a row, its part.
-template <class E, int D, int NB>
-__device__ __forceinline__ void cache_store(const CacheAttnParams& p, const CacheRows<E, D, NB>& a,
-                                            const CachePlan& c, int b, int hk, int v, int split,
-                                            int g) {
-  if (v >= p.G * p.M) return;
-  const int i = v / p.G, h = hk * p.G + (v - i * p.G);
-  const bool live = i < c.cnt;
-  const float l = xor32_add(a.l);
-  constexpr int DB = CacheRows<E, D, NB>::DB;
-  if (c.used > 1) {
-    const int64_t row = ((int64_t)(b * p.Hk + hk) * p.nsplit + split) * p.Rpad + v;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int d0 = 32 * db + 16 * hf + 8 * g;
-        if (d0 < D) {
-          const f32x16& o = a.o[db];
-          const int r = 8 * hf;
-          float* out = p.part_o + row * D + d0;
-          *reinterpret_cast<f32x4*>(out) = f32x4{o[r], o[r + 1], o[r + 2], o[r + 3]};
-          *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[r + 4], o[r + 5], o[r + 6], o[r + 7]};
-        }
-      }
-    if (g == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * row) =
-        f32x2{a.m == neg_inf() ? neg_inf() : a.m * p.qk_scale, l};
-    return;
-  }
-  const float inv = !live || l == 0.f ? 0.f : 1.f / l;
-  uint16_t* out = p.o + b * p.so0 + h * p.so1 + (int64_t)i * p.so2;
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int d0 = 32 * db + 16 * hf + 8 * g;
-      if (d0 < D) {
-        const f32x16& o = a.o[db];
-        const int r = 8 * hf;
-        // (A select: a padding row's lanes may hold infinities.)
-        const u32x4 w = {E::pack(o[r] * inv, o[r + 1] * inv), E::pack(o[r + 2] * inv, o[r + 3] * inv),
-                         E::pack(o[r + 4] * inv, o[r + 5] * inv),
-                         E::pack(o[r + 6] * inv, o[r + 7] * inv)};
-        *reinterpret_cast<u32x4*>(out + d0) = live ? w : u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-  if (g == 0 && p.lse != nullptr)
-    p.lse[b * p.sl0 + h * p.sl1 + (int64_t)i * p.sl2] =
-        !live || l == 0.f ? neg_inf()
-                          : (a.m * p.qk_scale + log2f_fast(l)) * 0.69314718055994531f;
-}
-
-// Q row of virtual row v from channel d0 on (zeros for rows that do not exist).
-template <int D>
-__device__ __forceinline__ u32x4 cache_q(const CacheAttnParams& p, int b, int hk, int v, int d0) {
-  const int i = v / p.G, h = hk * p.G + (v - i * p.G);
-  if (v >= p.G * p.M) return u32x4{0u, 0u, 0u, 0u};
-  return *reinterpret_cast<const u32x4*>(p.q + b * p.sq0 + h * p.sq1 + (int64_t)i * p.sq2 + d0) ^
-         p.qneg;
-}
 
 // ---------------------------------------------------------------- few rows
 
@@ -272,10 +62,10 @@ struct HalfRow {
 };
 
 template <class E, int D, int BITS>
-__global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p) {
-  constexpr int NW = 4, BN = 32, KS = D / 16, DB = (D + 31) / 32;
+__global__ __launch_bounds__(256) void cache_few_kernel(const RowsParams p) {
+  constexpr int NW = 4, BN = kCacheFewKeys, KS = D / 16, DB = (D + 31) / 32;
   constexpr int kChunk0 = D / 16;  // 16-byte chunks of half a row of values
-  using Rows = CacheRows<E, D, 1>;
+  using Rows = SoftRows<E, D, 1>;
   union Lds {
     uint16_t v[NW][BN * D];
     float rows[NW / 2][Rows::kSaved];
@@ -287,7 +77,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p)
   const int lane = tid & 63, c = lane & 31, g = lane >> 5;
   const int split = (int)(blockIdx.x % (uint32_t)p.nsplit), bhk = (int)(blockIdx.x / (uint32_t)p.nsplit);
   const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  const CachePlan plan = cache_plan<32, BN>(p, b, 0);
+  const RowsPlan plan = rows_plan<kCacheFewRows, BN>(p, b, 0);
   if (split >= plan.used) return;
   const int t1 = min(plan.tiles, (split + 1) * plan.per);
 
@@ -296,18 +86,18 @@ __global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p)
   const int pos = min(plan.pos0 + c / p.G, plan.hi);
   u32x4 q[KS];
 #pragma unroll
-  for (int m = 0; m < KS; ++m) q[m] = cache_q<D>(p, b, hk, c, g * (D / 2) + 8 * m);
+  for (int m = 0; m < KS; ++m) q[m] = load_q<D>(p, b, hk, c, g * (D / 2) + 8 * m);
 
-  const uint8_t* kc = p.kc + b * p.skc0 + hk * p.skc1;
+  const uint8_t* kc = p.k + b * p.sk0 + hk * p.sk1;
   const uint8_t* ks = p.ks + b * p.sks0 + hk * p.sks1;
-  const uint8_t* vc = p.vc + b * p.svc0 + hk * p.svc1;
+  const uint8_t* vc = p.v + b * p.sv0 + hk * p.sv1;
   const uint8_t* vs = p.vs + b * p.svs0 + hk * p.svs1;
   HalfRow<D, BITS> kn, vn;
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const int k0 = plan.tile(t) * BN;
     const int64_t kr = min(k0 + perm_row(c), plan.len - 1), vr = min(k0 + c, plan.len - 1);
-    kn.load(kc + kr * p.skc2, ks + kr * p.sks2, g);
-    vn.load(vc + vr * p.svc2, vs + vr * p.svs2, g);
+    kn.load(kc + kr * p.sk2, ks + kr * p.sks2, g);
+    vn.load(vc + vr * p.sv2, vs + vr * p.svs2, g);
   };
   Rows a;
   uint16_t* vt = lds.v[wave];
@@ -321,10 +111,10 @@ __global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p)
     f32x16 s[1] = {f32x16{}};
 #pragma unroll
     for (int m = 0; m < KS; ++m) s[0] = E::mma(kr.template get<E>(m), q[m], s[0]);
-    if (!cache_full(p, plan, k0, BN)) {
+    if (!rows_full(p, plan, k0, BN)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (!cache_sees(p, pos, k0 + acc_row(r, g))) s[0][r] = neg_inf();
+        if (!row_sees(p, pos, k0 + acc_row(r, g))) s[0][r] = neg_inf();
     }
     // This lane's NaN blocks as bits of the row's blocks.
     uint32_t nan = 0;
@@ -363,7 +153,7 @@ __global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p)
       for (int cs = 0; cs < 2; ++cs)
         a.o[db] = E::mma(lds_vt_operand<D>(vt, db, cs, lane), pb[cs], a.o[db]);
     if (any_nan)
-      cache_set_nan(a, p, pos, k0, [&](int row) {
+      set_nan_rows(a, p, pos, k0, [&](int row) {
         return (uint32_t)(__builtin_amdgcn_readlane((int)nan, row) |
                           __builtin_amdgcn_readlane((int)nan, row + 32));
       });
@@ -378,53 +168,44 @@ __global__ __launch_bounds__(256) void cache_few_kernel(const CacheAttnParams p)
   __syncthreads();
   if (wave != 0) return;
   a.add(lds.rows[0], lane, p.qk_scale);
-  cache_store<E, D, 1>(p, a, plan, b, hk, c, split, g);
+  store_rows<E, D, 1>(p, a, plan, b, hk, c, split, g);
 }
 
 // ---------------------------------------------------------------- many rows
 
+// Tiles of 64 cache rows for rows_kernel: 256 threads, each with a run of up to
+// 32 channels of one row.
 template <class E, int D, int BITS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void cache_rows_kernel(const CacheAttnParams p) {
-  constexpr int NW = 4, BM = 32 * NW, BN = 64, KS = D / 16, DB = (D + 31) / 32;
-  constexpr int TILE = BN * D;
-  constexpr int UPT = D >= 32 ? D / 32 : 1;  // units of 8 channels a thread converts
-  constexpr int UPR = D / 8;                 // units per row
-  constexpr int WPT = UPT * BITS / 4;        // words of codes
-  constexpr int GROUPS = D >= 32 ? D / 32 : 1;
-  __shared__ __attribute__((aligned(16))) uint16_t kv[2][2][TILE];
-  __shared__ __attribute__((aligned(4))) uint8_t nanb[2][BN][4];
-
-  const int tid = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = tid & 63, c = lane & 31, g = lane >> 5;
-  uint32_t id = blockIdx.x;
-  const int split = (int)(id % (uint32_t)p.nsplit);
-  id /= (uint32_t)p.nsplit;
-  const int nbh = p.B * p.Hk;
-  const int bhk = (int)(id % (uint32_t)nbh);
-  const int rb = p.nrb - 1 - (int)(id / (uint32_t)nbh);  // longest first
-  const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  const CachePlan plan = cache_plan<BM, BN>(p, b, rb);
-  if (split >= plan.used) return;
-  const int t0 = split * plan.per, t1 = min(plan.tiles, t0 + plan.per);
-
-  const int row0 = rb * BM + 32 * wave, v = row0 + c;
-  const int pos = min(plan.pos0 + v / p.G, plan.hi);
-  // Positions of the wave's live rows: it skips tiles that none of them sees.
-  const int wlo = plan.pos0 + row0 / p.G, whi = min(plan.pos0 + (row0 + 31) / p.G, plan.hi);
-  u32x4 q[KS];
-#pragma unroll
-  for (int m = 0; m < KS; ++m) q[m] = cache_q<D>(p, b, hk, v, 16 * m + 8 * g);
-
-  const int unit0 = tid * UPT, trow = unit0 / UPR, tunit = unit0 % UPR;
-  const bool stager = D >= 32 || tid < BN * UPR;
-  const uint8_t* kc = p.kc + b * p.skc0 + hk * p.skc1 + tunit * BITS;
-  const uint8_t* ks = p.ks + b * p.sks0 + hk * p.sks1 + tunit / 4;
-  const uint8_t* vc = p.vc + b * p.svc0 + hk * p.svc1 + tunit * BITS;
-  const uint8_t* vs = p.vs + b * p.svs0 + hk * p.svs1 + tunit / 4;
+struct CacheSource {
+  static constexpr bool kNanBlocks = true;
+  static constexpr int TILE = kRowsKeys * D;
+  static constexpr int UPT = D >= 32 ? D / 32 : 1;  // units of 8 channels a thread converts
+  static constexpr int UPR = D / 8;                 // units per row
+  static constexpr int WPT = UPT * BITS / 4;        // words of codes
+  static constexpr int GROUPS = D >= 32 ? D / 32 : 1;
+  struct Lds {
+    uint16_t kv[2][2][TILE];
+    uint8_t nan[2][kRowsKeys][4];
+  };
+  Lds& lds;
+  const RowsPlan& plan;
+  const int row, unit;
+  const bool stager;
+  const uint8_t *kc, *ks, *vc, *vs;
+  const int64_t skc, sks, svc, svs;
   uint32_t kw[WPT], vw[WPT], ksb = 0, vsb = 0;
-  auto words = [&](uint32_t (&w)[WPT], const uint8_t* src) __attribute__((always_inline)) {
+
+  __device__ __forceinline__ CacheSource(const RowsParams& p, const RowsPlan& plan_, int b, int hk,
+                                         Lds& lds_)
+      : lds(lds_), plan(plan_), row((int)threadIdx.x * UPT / UPR), unit((int)threadIdx.x * UPT % UPR),
+        stager(D >= 32 || (int)threadIdx.x < kRowsKeys * UPR),
+        kc(p.k + b * p.sk0 + hk * p.sk1 + unit * BITS),
+        ks(p.ks + b * p.sks0 + hk * p.sks1 + unit / 4),
+        vc(p.v + b * p.sv0 + hk * p.sv1 + unit * BITS),
+        vs(p.vs + b * p.svs0 + hk * p.svs1 + unit / 4),
+        skc(p.sk2), sks(p.sks2), svc(p.sv2), svs(p.svs2) {}
+
+  static __device__ __forceinline__ void words(uint32_t (&w)[WPT], const uint8_t* src) {
     if constexpr (WPT >= 4) {
 #pragma unroll
       for (int i = 0; i < WPT / 4; ++i) {
@@ -437,136 +218,38 @@ void cache_rows_kernel(const CacheAttnParams p) {
     } else {
       w[0] = *reinterpret_cast<const uint32_t*>(src);
     }
-  };
-  auto fetch = [&](int t) __attribute__((always_inline)) {
+  }
+  __device__ __forceinline__ void fetch(int t, int) {
     if (!stager) return;
-    const int64_t r = min(plan.tile(t) * BN + trow, plan.len - 1);
-    words(kw, kc + r * p.skc2);
-    words(vw, vc + r * p.svc2);
-    ksb = ks[r * p.sks2];
-    vsb = vs[r * p.svs2];
-  };
-  auto stash = [&](int stage) __attribute__((always_inline)) {
+    const int64_t r = min(plan.tile(t) * kRowsKeys + row, plan.len - 1);
+    words(kw, kc + r * skc);
+    words(vw, vc + r * svc);
+    ksb = ks[r * sks];
+    vsb = vs[r * svs];
+  }
+  __device__ __forceinline__ void land(int stage) {
     if (!stager) return;
     const bool nan = vsb == 0xffu;
     const float fk = cache_scale(ksb), fv = cache_scale(nan ? 0x7fu : vsb);
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
-      *reinterpret_cast<u32x4*>(&kv[stage][0][tile_off<D>(trow, tunit + i)]) =
+      const int off = tile_off<D>(row, unit + i);
+      *reinterpret_cast<u32x4*>(&lds.kv[stage][0][off]) =
           cache_unpack8<E, BITS>(kw + i * BITS / 4, fk);
       const u32x4 x = cache_unpack8<E, BITS>(vw + i * BITS / 4, fv);
-      *reinterpret_cast<u32x4*>(&kv[stage][1][tile_off<D>(trow, tunit + i)]) =
-          nan ? u32x4{0u, 0u, 0u, 0u} : x;
+      *reinterpret_cast<u32x4*>(&lds.kv[stage][1][off]) = nan ? u32x4{0u, 0u, 0u, 0u} : x;
     }
-    // (Where a block spans two threads, D = 16, both write the same byte.)
-    nanb[stage][trow][tunit / 4] = nan ? 1 : 0;
-    if (GROUPS < 4 && tunit == 0)
-      for (int i = GROUPS; i < 4; ++i) nanb[stage][trow][i] = 0;
-  };
-
-  CacheRows<E, D, 2> a;
-  if (t0 < t1) {
-    fetch(t0);
-    stash(0);
+    // (Where a block spans two threads both write the same byte.)
+    lds.nan[stage][row][unit / 4] = nan ? 1 : 0;
+    if (GROUPS < 4 && unit == 0)
+      for (int i = GROUPS; i < 4; ++i) lds.nan[stage][row][i] = 0;
   }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int stage = (t - t0) & 1, k0 = plan.tile(t) * BN;
-    if (t + 1 < t1) fetch(t + 1);
-    if (whi >= 0 && k0 <= whi && (k0 + BN > wlo - p.window + 1 || k0 < p.sinks)) {
-      const uint16_t *kt = kv[stage][0], *vt = kv[stage][1];
-      f32x16 s[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-      for (int m = 0; m < KS; ++m) {
-        s[0] = E::mma(lds_row_chunk<D>(kt, perm_row(c), m, g), q[m], s[0]);
-        s[1] = E::mma(lds_row_chunk<D>(kt, 32 + perm_row(c), m, g), q[m], s[1]);
-      }
-      if (!(k0 + BN - 1 <= wlo && (k0 > whi - p.window || k0 + BN <= p.sinks))) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!cache_sees(p, pos, k0 + 32 * kb + acc_row(r, g))) s[kb][r] = neg_inf();
-      }
-      u32x4 pb[4];
-      a.tile(s, p.qk_scale, pb);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int cs = 0; cs < 4; ++cs)
-          a.o[db] = E::mma(lds_vt_operand<D>(vt, db, cs, lane), pb[cs], a.o[db]);
-      uint32_t nan = *reinterpret_cast<const uint32_t*>(nanb[stage][lane]);
-      if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
-        nan = (nan & 1u) | ((nan >> 7) & 2u) | ((nan >> 14) & 4u) | ((nan >> 21) & 8u);
-        cache_set_nan(a, p, pos, k0,
-                      [&](int row) { return (uint32_t)__builtin_amdgcn_readlane((int)nan, row); });
-      }
-    }
-    if (t + 1 < t1) stash(stage ^ 1);
-    __syncthreads();
+  __device__ __forceinline__ const uint16_t* keys(int stage) const { return lds.kv[stage][0]; }
+  __device__ __forceinline__ const uint16_t* values(int stage) const { return lds.kv[stage][1]; }
+  __device__ __forceinline__ uint32_t nan_blocks(int stage, int lane) const {
+    const uint32_t n = *reinterpret_cast<const uint32_t*>(lds.nan[stage][lane]);
+    return (n & 1u) | ((n >> 7) & 2u) | ((n >> 14) & 4u) | ((n >> 21) & 8u);
   }
-  cache_store<E, D, 2>(p, a, plan, b, hk, v, split, g);
-}
-
-// ---------------------------------------------------------------- merge
-
-// Row v of KV head bhk: offset M = max of the parts' offsets, weights
-// 2^(m - M), L = sum w l, O = sum w O / L.  One workgroup a row: thread s holds
-// part s's weight, then 1024 / D threads share the parts of each group of four
-// channels.
-template <class E, int D, int BM, int BN>
-__global__ __launch_bounds__(256) void cache_merge_kernel(const CacheAttnParams p) {
-  constexpr int CH = D / 4, WAYS = 256 / CH;
-  __shared__ float wgt[kCacheMaxSplits];
-  __shared__ float red[2][4];
-  __shared__ f32x4 part[WAYS][CH];
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int rows = p.G * p.M;
-  const int bhk = (int)(blockIdx.x / (uint32_t)rows), v = (int)(blockIdx.x - (uint32_t)bhk * (uint32_t)rows);
-  const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  const CachePlan plan = cache_plan<BM, BN>(p, b, v / BM);
-  if (plan.used == 1) return;
-  const int64_t row0 = (int64_t)bhk * p.nsplit * p.Rpad + v;
-  static_assert(kCacheMaxSplits == 256, "one part a thread");
-  f32x2 ml{neg_inf(), 0.f};
-  if (tid < plan.used) ml = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * (row0 + (int64_t)tid * p.Rpad));
-  float mx = ml.x;
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-  if ((tid & 63) == 0) red[0][wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float w = ml.x == neg_inf() ? 0.f : exp2f_fast(ml.x - mx);
-  wgt[tid] = w;
-  // (A part without an offset has l = 0, or NaN where its scores were.)
-  float l = ml.x == neg_inf() ? ml.y : w * ml.y;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i);
-  if ((tid & 63) == 0) red[1][wave] = l;
-  __syncthreads();
-  l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const int ch = tid % CH, way = tid / CH;
-  f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = way; s < plan.used; s += WAYS) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + (row0 + (int64_t)s * p.Rpad) * D + 4 * ch);
-    const float ws = wgt[s];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(ws, x[e], acc[e]);
-  }
-  part[way][ch] = acc;
-  __syncthreads();
-  if (way != 0) return;
-  for (int s = 1; s < WAYS; ++s) acc += part[s][ch];
-  const int i = v / p.G, h = hk * p.G + (v - i * p.G);
-  const bool live = i < plan.cnt;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<u32x2*>(p.o + b * p.so0 + h * p.so1 + (int64_t)i * p.so2 + 4 * ch) =
-      live ? u32x2{E::pack(acc[0] * inv, acc[1] * inv), E::pack(acc[2] * inv, acc[3] * inv)}
-           : u32x2{0u, 0u};
-  if (ch == 0 && p.lse != nullptr)
-    p.lse[b * p.sl0 + h * p.sl1 + (int64_t)i * p.sl2] =
-        !live || l == 0.f ? neg_inf() : (mx + log2f_fast(l)) * 0.69314718055994531f;
-}
+};
 
 }  // namespace fas

@@ -52,12 +52,27 @@ inline int check_tensor(const char* fn, const char* name, const void* ptr, const
   return FAS_OK;
 }
 
+constexpr int64_t kCus = 256;  // MI355X compute units
+
 // Compute units of the current device (fas_api.cpp).
 int device_cu_count();
 
 inline uint32_t slice_bytes(int64_t rows, int64_t row_stride, int64_t D) {
   return rows <= 0 ? 0u : (uint32_t)(((rows - 1) * row_stride + D) * 2);
 }
+
+struct Problem {
+  int B, H, Hk, G, M, N, D, dtype, causal;
+  bool dropout;  // dropout_p > 0
+  bool keep;     // dropout with a caller keep-bit buffer (fas_attn_args.keep_bits)
+  float sm_scale;
+  int pack;  // query heads per forward workgroup (GQA packing): G, or 1
+};
+
+// Sizes, dtype and flags of a request (no pointers), and with its tensors
+// (fas_api.cpp).
+int check_shape(const char* fn, const fas_attn_args* a, Problem* pr);
+int check_args(const char* fn, const fas_attn_args* a, Problem* pr);
 
 // Exponent scale of the base-2 softmax, |sm_scale| * log2(e).  For
 // sm_scale == 0 the weights are uniform over the admissible keys; a zero

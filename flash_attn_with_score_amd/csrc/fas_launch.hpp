@@ -45,10 +45,11 @@ hipError_t launch_fill_zero(float* p, int64_t s0, int64_t s1, int64_t s2, int64_
 // Quantised KV cache (fas_cache.hpp, fas_cache_attn.hpp).
 hipError_t launch_cache_append(const CacheParams& p, int dtype, int d, int bits, hipStream_t s);
 hipError_t launch_cache_read(const CacheParams& p, int dtype, int d, int bits, hipStream_t s);
-hipError_t launch_cache_attn(const CacheAttnParams& p, int dtype, int d, int bits, hipStream_t s);
-// Most virtual rows of cache_few_kernel, and a block of cache_rows_kernel; their
-// key tiles.
-constexpr int kCacheFewRows = 32, kCacheBlockRows = 128;
-constexpr int kCacheFewKeys = 32, kCacheBlockKeys = 64;
+hipError_t launch_cache_attn(const RowsParams& p, int dtype, int d, int bits, hipStream_t s);
+
+// Windowed attention over dense keys (fas_window.hpp) and its backward: prep,
+// dK/dV (+ reduction), dQ.
+hipError_t launch_window_fwd(const RowsParams& p, int dtype, int d, hipStream_t s);
+hipError_t launch_window_bwd(const WindowBwdParams& p, int dtype, int d, hipStream_t s);
 
 }  // namespace fas

@@ -318,28 +318,38 @@ struct CacheParams {
   int chunks;              // workgroups per tensor, batch entry and head
 };
 
-// Most workgroups that share a row's keys (cache_merge_kernel holds one part a
-// thread).
-constexpr int kCacheMaxSplits = 256;
+}  // namespace fas
 
-// Attention over the quantised cache (fas_cache_attn.hpp).
-struct CacheAttnParams {
+namespace fas {
+
+// Most workgroups that share a row's keys (merge_kernel holds one part a
+// thread).
+constexpr int kRowsMaxSplits = 256;
+// Virtual rows of cache_few_kernel and of a rows_kernel block; their key tiles.
+constexpr int kCacheFewRows = 32, kRowsBlock = 128;
+constexpr int kCacheFewKeys = 32, kRowsKeys = 64;
+
+// Attention with a window and sinks over dense keys or the quantised cache
+// (fas_rows.hpp).
+struct RowsParams {
   const uint16_t* q;
   uint16_t* o;
   float* lse;              // optional (B, H, M)
-  const uint8_t *kc, *ks, *vc, *vs;
-  int64_t sq0, sq1, sq2;
+  const uint8_t *k, *v;    // dense rows, or codes
+  const uint8_t *ks, *vs;  // the codes' scales
+  int64_t sq0, sq1, sq2;   // q, o, lse: strides in elements
   int64_t so0, so1, so2;
   int64_t sl0, sl1, sl2;
-  int64_t skc0, skc1, skc2, sks0, sks1, sks2;
-  int64_t svc0, svc1, svc2, svs0, svs1, svs2;
+  int64_t sk0, sk1, sk2, sks0, sks1, sks2;  // k, v and scales: in bytes
+  int64_t sv0, sv1, sv2, svs0, svs1, svs2;
+  uint32_t k_bytes, v_bytes;  // dense: extents of a head's keys and values
   const int32_t* lengths;  // (B,) or null: lengths_all
   const int32_t* counts;   // (B,) or null: M
   int lengths_all;
   int B, H, Hk, G, M, capacity;
-  int window, sinks;       // window at most kCacheNoWindow
-  int nrb;                 // cache_rows_kernel: blocks of 128 virtual rows
-  int nsplit;              // workgroups per row block, at most kCacheMaxSplits
+  int window, sinks;       // window at most kNoWindow
+  int nrb;                 // blocks of virtual rows
+  int nsplit;              // workgroups per row block, at most kRowsMaxSplits
   int min_tiles;           // least key tiles of a workgroup
   int Rpad;                // virtual rows, padded to whole blocks
   float* part_o;           // (B * Hk, nsplit, Rpad, D): unnormalised O
@@ -348,6 +358,16 @@ struct CacheAttnParams {
   uint32_t qneg;           // 0x80008000 to negate q (negative sm_scale), else 0
 };
 // Window of a call without one; pos - window stays inside 32 bits.
-constexpr int kCacheNoWindow = 1 << 30;
+constexpr int kNoWindow = 1 << 30;
+
+// Backward of the windowed attention (fas_window.hpp).  part: fp32 dK | dV of
+// the key blocks dealt to several workgroups, slabs of 128 keys x 2D: first
+// the `sink_blocks` blocks that hold sinks (seen by every later row), in
+// sink_pieces each, then the others in `pieces` each where that is more than
+// one.
+struct WindowBwdParams : BwdParams {
+  int window, sinks;
+  int sink_blocks, sink_pieces;
+};
 
 }  // namespace fas

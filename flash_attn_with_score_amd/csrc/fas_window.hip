@@ -1,0 +1,71 @@
+// Instances and launchers of the windowed attention (fas_window.hpp).
+#include "fas_launch.hpp"
+#include "fas_window.hpp"
+
+namespace fas {
+
+template <class E, int D>
+static hipError_t fwd_t(const RowsParams& p, hipStream_t s) {
+  const dim3 block(256);
+  hipLaunchKernelGGL((rows_kernel<E, D, DenseSource<E, D>>),
+                     dim3((unsigned)((int64_t)p.B * p.Hk * p.nrb * p.nsplit)), block, 0, s, p);
+  if (p.nsplit > 1)
+    hipLaunchKernelGGL((merge_kernel<E, D, kRowsBlock, kRowsKeys>),
+                       dim3((unsigned)((int64_t)p.B * p.H * p.M)), block, 0, s, p);
+  return hipGetLastError();
+}
+
+template <class E, int D>
+static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
+  const int64_t bh = (int64_t)p.B * p.H, bhk = (int64_t)p.B * p.Hk;
+  if (p.M > 0)
+    hipLaunchKernelGGL((bwd_prep_kernel<E, D>), dim3((unsigned)(bh * p.nprep)), dim3(256), 0, s,
+                       p);
+  if (p.N > 0) {
+    const int64_t items = (int64_t)p.sink_blocks * p.sink_pieces +
+                          (int64_t)(p.nkb - p.sink_blocks) * p.pieces;
+    hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)(bhk * items)), dim3(256), 0, s,
+                       p);
+    if (p.pieces > 1 || p.sink_pieces > 1) {
+      const int nkeys = p.pieces > 1 ? p.N : p.sink_blocks * kBwdBlock < p.N
+                                                 ? p.sink_blocks * kBwdBlock : p.N;
+      const int64_t blocks = (bhk * nkeys * (D / 8) + 255) / 256;
+      hipLaunchKernelGGL((window_reduce_kernel<E, D>),
+                         dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, p,
+                         nkeys);
+    }
+  }
+  if (p.M > 0)
+    hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)(bh * p.nrb)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+template <class E>
+static hipError_t fwd_d(const RowsParams& p, int d, hipStream_t s) {
+  switch (d) {
+    case 16: return fwd_t<E, 16>(p, s);
+    case 32: return fwd_t<E, 32>(p, s);
+    case 64: return fwd_t<E, 64>(p, s);
+    case 128: return fwd_t<E, 128>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+template <class E>
+static hipError_t bwd_d(const WindowBwdParams& p, int d, hipStream_t s) {
+  switch (d) {
+    case 16: return bwd_t<E, 16>(p, s);
+    case 32: return bwd_t<E, 32>(p, s);
+    case 64: return bwd_t<E, 64>(p, s);
+    case 128: return bwd_t<E, 128>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_window_fwd(const RowsParams& p, int dtype, int d, hipStream_t s) {
+  return dtype == 0 ? fwd_d<F16>(p, d, s) : fwd_d<BF16>(p, d, s);
+}
+hipError_t launch_window_bwd(const WindowBwdParams& p, int dtype, int d, hipStream_t s) {
+  return dtype == 0 ? bwd_d<F16>(p, d, s) : bwd_d<BF16>(p, d, s);
+}
+
+}  // namespace fas

@@ -1,0 +1,488 @@
+// gfx950 windowed attention over dense keys, forward (rows_kernel of
+// fas_rows.hpp with DenseSource) and backward.
+//
+// Query row i is at position p = (N - M) + i and sees key j iff j <= p and
+// (j > p - window or j < sinks).  The backward has attention()'s three passes
+// (fas_bwd.hpp: the operand layouts) over the visible pairs alone:
+//
+//   bwd_prep_kernel       per row: -delta = -sum_d O dO and -L log2(e)
+//   window_dkdv_kernel    key-block outer: S, P, dP, dS, dV^T += dO^T P,
+//                         dK^T += Q^T dS.  The rows that see a block of 128
+//                         keys are one run: those at most `window` behind its
+//                         last key, or, where the block holds sinks, all later
+//                         ones.  A block with sinks would take M / (window +
+//                         128) times as long as another, so its run is dealt
+//                         to as many workgroups as make them about equal;
+//                         they write fp32 parts that window_reduce_kernel
+//                         adds in order.
+//   window_dq_kernel      query-block outer: tiles of 64 keys, the sinks' first,
+//                         then the window's: S^T, P^T, dS^T, dQ^T += K^T dS^T.
+//
+// A pair that a row does not see has P = 0 and so dS = 0; P and dS are rounded
+// to the input type for their products, everything else is fp32.
+#pragma once
+#include "fas_bwd.hpp"
+#include "fas_rows.hpp"
+
+namespace fas {
+
+// Tiles of 64 dense rows by LDS DMA (rows past the last key read as zeros).
+template <class E, int D>
+struct DenseSource {
+  static constexpr bool kNanBlocks = false;
+  static constexpr int TILE = kRowsKeys * D;
+  struct Lds {
+    uint16_t kv[2][2][TILE];
+  };
+  Lds& lds;
+  const RowsPlan& plan;
+  const i32x4 wk_, wv_;
+  const int64_t sk, sv;
+  const int wave, lane;
+  static __device__ __forceinline__ i32x4 uniform(i32x4 w) {
+    return i32x4{__builtin_amdgcn_readfirstlane(w.x), __builtin_amdgcn_readfirstlane(w.y),
+                 __builtin_amdgcn_readfirstlane(w.z), __builtin_amdgcn_readfirstlane(w.w)};
+  }
+  __device__ __forceinline__ DenseSource(const RowsParams& p, const RowsPlan& plan_, int b, int hk,
+                                         Lds& lds_)
+      : lds(lds_), plan(plan_),
+        wk_(make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes)),
+        wv_(make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes)), sk(p.sk2 >> 1),
+        sv(p.sv2 >> 1), wave(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)),
+        lane((int)threadIdx.x & 63) {}
+  __device__ __forceinline__ void fetch(int t, int stage) {
+    const int r0 = plan.tile(t) * kRowsKeys;
+    // (The descriptors are uniform, but at D = 16, where half the waves load,
+    // the compiler moves them to vector registers.)
+    const i32x4 wk = uniform(wk_), wv = uniform(wv_);
+    dma_tile<D, kRowsKeys, 4>(wk, sk, r0, lds_addr(lds.kv[stage][0]), wave, lane);
+    dma_tile<D, kRowsKeys, 4>(wv, sv, r0, lds_addr(lds.kv[stage][1]), wave, lane);
+  }
+  __device__ __forceinline__ void land(int) { vm_wait_all(); }
+  __device__ __forceinline__ const uint16_t* keys(int stage) const { return lds.kv[stage][0]; }
+  __device__ __forceinline__ const uint16_t* values(int stage) const { return lds.kv[stage][1]; }
+};
+
+// Part of the fp32 workspace that piece `piece` of key block kb writes.
+__device__ __forceinline__ int64_t window_slab(const WindowBwdParams& p, int bhk, int kb, int piece) {
+  if (kb < p.sink_blocks) return ((int64_t)bhk * p.sink_blocks + kb) * p.sink_pieces + piece;
+  const int64_t base = p.sink_pieces > 1 ? (int64_t)p.B * p.Hk * p.sink_blocks * p.sink_pieces : 0;
+  return base + ((int64_t)bhk * (p.nkb - p.sink_blocks) + kb - p.sink_blocks) * p.pieces + piece;
+}
+
+// ---------------------------------------------------------------- dK, dV
+
+template <class E, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 2 : 1)))
+void window_dkdv_kernel(const WindowBwdParams p) {
+  constexpr int KS = D / 16;
+  constexpr int DB = D >= 32 ? D / 32 : 1;
+  constexpr int NW = 4;
+  constexpr int BK = 32 * NW;  // keys per workgroup
+  constexpr int TQ = 64;       // query rows per tile
+  constexpr int TILE = TQ * D;
+
+  __shared__ __attribute__((aligned(16))) uint16_t qlds[2][TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t glds[2][TILE];  // dO
+  __shared__ __attribute__((aligned(16))) float nlds[2][TQ];
+  __shared__ __attribute__((aligned(16))) float xlds[2][TQ];       // -delta
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 31, g = lane >> 5;
+  // The sinks' pieces first, then the other blocks'.
+  const int nbh = p.B * p.Hk;
+  int id = blockIdx.x, kb, pieces = p.sink_pieces;
+  const int nsink = p.sink_blocks * pieces * nbh;
+  if (id >= nsink) {
+    id -= nsink;
+    pieces = p.pieces;
+    kb = p.sink_blocks + id / (nbh * pieces);
+  } else {
+    kb = id / (nbh * pieces);
+  }
+  const int rest = id % (nbh * pieces);
+  const int piece = rest % pieces, bhk = rest / pieces;
+  const int b = bhk / p.Hk, hk = bhk % p.Hk;
+  const int h0 = hk * p.G;
+  const int key0 = kb * BK + 32 * wave;  // this wave's keys [key0, key0 + 32)
+
+  const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
+  const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
+  u32x4 kreg[KS], vreg[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    kreg[ks] = buf_load16(rk, (uint32_t)(((key0 + c) * p.sk2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
+    vreg[ks] = buf_load16(rv, (uint32_t)(((key0 + c) * p.sv2 + 16 * ks + 8 * g) * 2));
+  }
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kreg[ks]), "+v"(vreg[ks]));
+
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    dk[db] = f32x16{};
+    dv[db] = f32x16{};
+  }
+
+  // Query rows [rlo, rhi) that see a key of the block.
+  const int rlo = max(0, kb * BK - p.causal_off);
+  const int rhi = kb * BK < p.sinks ? p.M
+                                    : min((int64_t)p.M, (int64_t)kb * BK + BK - 1 + p.window - p.causal_off);
+  const int tlo = rlo / TQ, tiles = max(0, (rhi + TQ - 1) / TQ - tlo);
+  // This piece's tiles [s0, s1) of the G heads' tiles in head order.
+  int s0, s1;
+  deal(p.G * tiles, piece, pieces, s0, s1);
+  s1 += s0;
+  const float qk = p.qk_scale;
+  const uint32_t q_base = lds_addr(&qlds[0][0]), g_base = lds_addr(&glds[0][0]);
+  // Row position - key, per lane: a row sees key key0 + c iff 0 <= difference
+  // < reach (a key past N: never).
+  const int reach = key0 + c >= p.N ? 0 : key0 + c < p.sinks ? 0x7fffffff : p.window;
+
+  for (int hh = 0; hh < p.G; ++hh) {
+    const int t0 = tlo + max(0, s0 - hh * tiles), t1 = tlo + min(tiles, s1 - hh * tiles);
+    if (t0 >= t1) continue;
+    const int h = h0 + hh;
+    const int64_t bh = (int64_t)b * p.H + h;
+    const i32x4 wq = make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes);
+    const i32x4 wg = make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
+    const float* nlg = p.nl + bh * p.Mpad;
+    const float* xg = p.delta + bh * p.Mpad;
+    float nst = 0.f, xst = 0.f;
+    auto fetch = [&](int t, int s) __attribute__((always_inline)) {
+      dma_tile<D, TQ, NW>(wq, p.sq2, t * TQ, q_base + (uint32_t)(s * TILE * 2), wave, lane);
+      dma_tile<D, TQ, NW>(wg, p.sg2, t * TQ, g_base + (uint32_t)(s * TILE * 2), wave, lane);
+      if (tid < TQ) {
+        nst = nlg[t * TQ + tid];
+        xst = xg[t * TQ + tid];
+      }
+    };
+    auto stash = [&](int s) __attribute__((always_inline)) {
+      if (tid < TQ) {
+        nlds[s][tid] = nst;
+        xlds[s][tid] = xst;
+      }
+    };
+    fetch(t0, 0);
+    vm_wait_all();
+    stash(0);
+    __syncthreads();
+    auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
+      constexpr int stage = decltype(stage_tag)::value;
+      const bool more = t + 1 < t1;
+      if (more) fetch(t + 1, stage ^ 1);
+      const uint16_t* qt = qlds[stage];
+      const uint16_t* gt = glds[stage];
+      // One 32-row block; masked and unmasked copies of the elementwise part
+      // join before the dV / dK products.
+      auto body = [&](int qb, bool full) __attribute__((always_inline)) {
+        const int r0 = t * TQ + 32 * qb;
+        // Register r holds query row r0 + acc_row(r, g) and key key0 + c.
+        f32x16 s = f32x16{}, dp;
+        load8(dp, &xlds[stage][32 * qb + 8 * g], 0, 0);
+        load8(dp, &xlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          s = E::mma(lds_row_chunk<D>(qt, 32 * qb + perm_row(c), ks, g), kreg[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          dp = E::mma(lds_row_chunk<D>(gt, 32 * qb + perm_row(c), ks, g), vreg[ks], dp);
+        f32x16 nl;
+        load8(nl, &nlds[stage][32 * qb + 8 * g], 0, 0);
+        load8(nl, &nlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2f_fast(fmaf(s[r], qk, nl[r]));
+        if (!full) {
+          const int diff = p.causal_off + r0 - (key0 + c);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((uint32_t)(diff + acc_row(r, g)) >= (uint32_t)reach) s[r] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+        const u32x4 pb0 = pack_b<E>(s, 0), pb1 = pack_b<E>(s, 1);
+        const u32x4 sb0 = pack_b<E>(dp, 0), sb1 = pack_b<E>(dp, 1);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          dv[db] = E::mma(lds_vt_operand<D>(gt, db, 2 * qb, lane), pb0, dv[db]);
+          dv[db] = E::mma(lds_vt_operand<D>(gt, db, 2 * qb + 1, lane), pb1, dv[db]);
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          dk[db] = E::mma(lds_vt_operand<D>(qt, db, 2 * qb, lane), sb0, dk[db]);
+          dk[db] = E::mma(lds_vt_operand<D>(qt, db, 2 * qb + 1, lane), sb1, dk[db]);
+        }
+      };
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        // Positions p0 .. p0 + 31 against the wave's keys.
+        const int p0 = p.causal_off + t * TQ + 32 * qb;
+        const bool live = p0 + 31 >= key0 && (key0 + 31 > p0 - p.window || key0 < p.sinks);
+        const bool full = p0 >= key0 + 31 && key0 + 31 < p.N &&
+                          (key0 > p0 + 31 - p.window || key0 + 32 <= p.sinks);
+        if (live) body(qb, full);
+      }
+      if (more) {
+        vm_wait_all();
+        stash(stage ^ 1);
+      }
+      __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+      step(t, std::integral_constant<int, 0>{});
+      if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
+    }
+  }
+
+  // Lane (c, g), register r of block db: key key0 + c, head dim
+  // 32db + acc_row(r, g).
+  const int key = key0 + c;
+  if (key >= p.N) return;
+  const float ks_ = p.scale_signed;
+  if (pieces == 1) {
+    uint16_t* dkr = p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2;
+    uint16_t* dvr = p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int d0 = 32 * db + 16 * hf + 8 * g;
+        if (d0 < D) {
+          f32x16 x = dk[db] * ks_;
+          *reinterpret_cast<u32x4*>(dkr + d0) = pack_b<E>(x, hf);
+          *reinterpret_cast<u32x4*>(dvr + d0) = pack_b<E>(dv[db], hf);
+        }
+      }
+  } else {
+    float* pr = p.part + (window_slab(p, bhk, kb, piece) * BK + 32 * wave + c) * (2 * D);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int d0 = 32 * db + 16 * hf + 8 * g;
+        if (d0 < D) {
+          const f32x16& x = dk[db];
+          const f32x16& y = dv[db];
+          const int r = 8 * hf;
+          *reinterpret_cast<f32x4*>(pr + d0) =
+              f32x4{x[r] * ks_, x[r + 1] * ks_, x[r + 2] * ks_, x[r + 3] * ks_};
+          *reinterpret_cast<f32x4*>(pr + d0 + 4) =
+              f32x4{x[r + 4] * ks_, x[r + 5] * ks_, x[r + 6] * ks_, x[r + 7] * ks_};
+          *reinterpret_cast<f32x4*>(pr + D + d0) = f32x4{y[r], y[r + 1], y[r + 2], y[r + 3]};
+          *reinterpret_cast<f32x4*>(pr + D + d0 + 4) =
+              f32x4{y[r + 4], y[r + 5], y[r + 6], y[r + 7]};
+        }
+      }
+  }
+}
+
+// dK, dV of the key blocks that were dealt to several workgroups: the sum of
+// their parts, in order.  One thread per 8 elements of keys [0, nkeys) of each
+// KV head: the sinks' blocks, or all of them.
+template <class E, int D>
+__global__ __launch_bounds__(256) void window_reduce_kernel(const WindowBwdParams p, int nkeys) {
+  constexpr int CPR = D / 8;
+  const int64_t total = (int64_t)p.B * p.Hk * nkeys * CPR;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int ch = (int)(i % CPR);
+    const int64_t r = i / CPR;
+    const int key = (int)(r % nkeys), bhk = (int)(r / nkeys);
+    const int kb = key / kBwdBlock, pieces = kb < p.sink_blocks ? p.sink_pieces : p.pieces;
+    if (pieces == 1) continue;  // written by its only workgroup
+    const int hk = bhk % p.Hk, b = bhk / p.Hk;
+    const float* src =
+        p.part + (window_slab(p, bhk, kb, 0) * kBwdBlock + key % kBwdBlock) * (2 * D) + 8 * ch;
+    float a[8] = {}, v[8] = {};
+#pragma unroll 4
+    for (int j = 0; j < pieces; ++j, src += kBwdBlock * 2 * D) {
+      const f32x4 a0 = *reinterpret_cast<const f32x4*>(src);
+      const f32x4 a1 = *reinterpret_cast<const f32x4*>(src + 4);
+      const f32x4 v0 = *reinterpret_cast<const f32x4*>(src + D);
+      const f32x4 v1 = *reinterpret_cast<const f32x4*>(src + D + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] += a0[e];
+        a[4 + e] += a1[e];
+        v[e] += v0[e];
+        v[4 + e] += v1[e];
+      }
+    }
+    const int d0 = 8 * ch;
+    *reinterpret_cast<u32x4*>(p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2 + d0) =
+        u32x4{E::pack(a[0], a[1]), E::pack(a[2], a[3]), E::pack(a[4], a[5]), E::pack(a[6], a[7])};
+    *reinterpret_cast<u32x4*>(p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2 + d0) =
+        u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
+  }
+}
+
+// ---------------------------------------------------------------- dQ
+
+template <class E, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void window_dq_kernel(const WindowBwdParams p) {
+  constexpr int KS = D / 16;
+  constexpr int DB = D >= 32 ? D / 32 : 1;
+  constexpr int NW = 4;
+  constexpr int BM = 32 * NW;  // query rows per workgroup
+  constexpr int BN = 64;       // keys per tile
+  constexpr int TILE = BN * D;
+
+  __shared__ __attribute__((aligned(16))) uint16_t klds[2][TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t vlds[2][TILE];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 31, g = lane >> 5;
+  const int nbh = p.B * p.H;
+  const int bh = blockIdx.x % nbh;
+  const int rb = p.nrb - 1 - blockIdx.x / nbh;  // longest row blocks first
+  const int b = bh / p.H, h = bh % p.H, hk = h / p.G;
+  const int row0 = rb * BM, wrow0 = row0 + 32 * wave, qrow = wrow0 + c;
+
+  const __amdgpu_buffer_rsrc_t rq = make_rsrc(p.q + b * p.sq0 + h * p.sq1, p.q_bytes);
+  const __amdgpu_buffer_rsrc_t rg = make_rsrc(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
+  u32x4 qreg[KS], greg[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    qreg[ks] = buf_load16(rq, (uint32_t)((qrow * p.sq2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
+    greg[ks] = buf_load16(rg, (uint32_t)((qrow * p.sg2 + 16 * ks + 8 * g) * 2));
+  }
+  // Rows past M read nl = -inf (padding), so their P is 0.
+  const float nl = p.nl[(int64_t)bh * p.Mpad + qrow];
+  const float xl = p.delta[(int64_t)bh * p.Mpad + qrow];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]), "+v"(greg[ks]));
+
+  // Key tiles of the block: the sinks' before the window, then the window's.
+  const int lo = p.causal_off + row0, hi = min(p.N - 1, lo + BM - 1);
+  int sink_tiles = 0, win = 0, ntiles = 0;
+  if (hi >= 0) {
+    win = max(0, lo - p.window + 1) / BN;
+    sink_tiles = min(win, (min(p.sinks, hi + 1) + BN - 1) / BN);
+    ntiles = sink_tiles + (hi + BN) / BN - win;
+  }
+  const int wlo = p.causal_off + wrow0, whi = wrow0 < p.M ? min(p.N - 1, wlo + 31) : -1;
+  const int pos = p.causal_off + qrow;
+
+  const i32x4 wk = make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
+  const i32x4 wv = make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
+  const uint32_t k_base = lds_addr(&klds[0][0]), v_base = lds_addr(&vlds[0][0]);
+  auto tile_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + win) * BN; };
+  auto fetch = [&](int t, int s) __attribute__((always_inline)) {
+    dma_tile<D, BN, NW>(wk, p.sk2, tile_key(t), k_base + (uint32_t)(s * TILE * 2), wave, lane);
+    dma_tile<D, BN, NW>(wv, p.sv2, tile_key(t), v_base + (uint32_t)(s * TILE * 2), wave, lane);
+  };
+
+  f32x16 dq[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
+  const float qk = p.qk_scale;
+  const VtOff vto = vt_offsets<D>(lane);
+  const uint32_t rco = row_chunk_offset<D>(perm_row(c), g);
+
+  if (ntiles > 0) {
+    fetch(0, 0);
+    vm_wait_all();
+    __syncthreads();
+  }
+  auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
+    constexpr int stage = decltype(stage_tag)::value;
+    const bool more = t + 1 < ntiles;
+    if (more) fetch(t + 1, stage ^ 1);
+    const uint16_t* kt = klds[stage];
+    const uint16_t* vt = vlds[stage];
+    const int k0 = tile_key(t);
+    // One 32-key sub-block (bwd_dq_kernel has the reasons for its fences).
+    auto body = [&](int kb2, bool full) __attribute__((always_inline)) {
+      const int kbase = k0 + 32 * kb2;
+      __builtin_amdgcn_sched_barrier(0);
+      uint32_t ro = rco;
+      opaque(ro);
+      u32x4 ak[KS], av[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        ak[ks] = lds_row_chunk(kt + 32 * kb2 * D, ro, ks);
+        av[ks] = lds_row_chunk(vt + 32 * kb2 * D, ro, ks);
+      }
+      // Register r holds key kbase + acc_row(r, g) for query row qrow.
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = xl;
+      s = E::mma(ak[0], qreg[0], f32x16{});
+      dp = E::mma(av[0], greg[0], dp);
+#pragma unroll
+      for (int ks = 1; ks < KS; ++ks) {
+        s = E::mma(ak[ks], qreg[ks], s);
+        dp = E::mma(av[ks], greg[ks], dp);
+      }
+      {
+        constexpr int PD = KS < 2 ? KS : 2;
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * PD, 0);  // DS read
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
+          if (i + PD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+      }
+      float pr[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pr[r] = exp2f_fast(fmaf(s[r], qk, nl));
+        if (!full) {
+          const int key = kbase + acc_row(r, g);
+          if (key > pos || (key <= pos - p.window && key >= p.sinks)) pr[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = pr[r] * dp[r];
+      const u32x4 sb0 = pack_b<E>(dp, 0), sb1 = pack_b<E>(dp, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      VtOff o = vto;
+      opaque(o);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dq[db] = E::mma(lds_vt_operand<D>(kt, o, db, 2 * kb2), sb0, dq[db]);
+        dq[db] = E::mma(lds_vt_operand<D>(kt, o, db, 2 * kb2 + 1), sb1, dq[db]);
+      }
+      {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * DB; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i + 2 < 2 * DB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+      }
+    };
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      const int kbase = k0 + 32 * kb2;
+      const bool live = kbase <= whi && (kbase + 32 > wlo - p.window + 1 || kbase < p.sinks);
+      const bool full = kbase + 31 <= wlo && (kbase > whi - p.window || kbase + 32 <= p.sinks);
+      if (live) body(kb2, full);
+    }
+    if (more) vm_wait_all();
+    __syncthreads();
+  };
+  for (int t = 0; t < ntiles; t += 2) {
+    step(t, std::integral_constant<int, 0>{});
+    if (t + 1 < ntiles) step(t + 1, std::integral_constant<int, 1>{});
+  }
+
+  // Lane (c, g), register r of block db: row qrow, head dim 32db + acc_row(r, g).
+  if (qrow >= p.M) return;
+  uint16_t* dqr = p.dq + b * p.sdq0 + h * p.sdq1 + (int64_t)qrow * p.sdq2;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int d0 = 32 * db + 16 * hf + 8 * g;
+      if (d0 < D) {
+        const f32x16 x = dq[db] * p.scale_signed;
+        *reinterpret_cast<u32x4*>(dqr + d0) = pack_b<E>(x, hf);
+      }
+    }
+}
+
+}  // namespace fas

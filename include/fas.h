@@ -281,6 +281,32 @@ int fas_attention_backward(const fas_attn_args* a, const void* dout,
                            const int64_t dv_stride[4], void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---- Attention with a sliding window and sinks.  No counterpart in the
+ * reference. ----
+ *
+ * As fas_attention_forward without dropout, under the mask: query row i, at
+ * position p = (seqlen_k - seqlen_q) + i, sees key j iff j <= p and
+ * (j > p - window or j < sinks).  a->causal must be 1, window at least 1;
+ * window >= seqlen_k is the causal mask.  Rows that see no key give out = 0 and
+ * lse = -inf.  lse (NULL: not wanted) is what the backward pass takes.  The
+ * workspace is fas_attention_window_workspace(a, window, sinks, 0) bytes,
+ * 256-byte aligned ((size_t)-1: invalid request). */
+size_t fas_attention_window_workspace(const fas_attn_args* a, int64_t window, int64_t sinks,
+                                      int backward);
+int fas_attention_window(const fas_attn_args* a, int64_t window, int64_t sinks, float* lse,
+                         const int64_t lse_stride[3], void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Its gradients, with the arguments of fas_attention_backward: a->out and lse as
+ * the forward wrote them, dk and dv summed in fp32 over the query heads of each
+ * KV head.  Workspace: fas_attention_window_workspace(a, window, sinks, 1). */
+int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_t sinks,
+                                  const void* dout, const int64_t dout_stride[4], const float* lse,
+                                  const int64_t lse_stride[3], void* dq, const int64_t dq_stride[4],
+                                  void* dk, const int64_t dk_stride[4], void* dv,
+                                  const int64_t dv_stride[4], void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* ---- Quantised KV cache.  No counterpart in the reference. ----
  *
  * The keys and values of a batch of sequences, (batch, heads, capacity,
