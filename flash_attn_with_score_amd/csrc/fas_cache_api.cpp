@@ -149,7 +149,7 @@ fas::RowsSplit attn_split(const fas_kv_cache* c, const fas_kv_query* a) {
   const int64_t rows = a->heads_q / c->heads * a->tokens;
   return fas::rows_split(c->batch * c->heads, rows, a->tokens,
                          a->lengths == nullptr ? a->lengths_all : c->capacity, a->window, a->sinks,
-                         c->head_dim, rows <= fas::kCacheFewRows);
+                         c->head_dim, rows <= fas::kFewRows);
 }
 
 }  // namespace

@@ -1,27 +1,13 @@
 // Instances and launcher of the attention over the quantised KV cache
 // (fas_cache_attn.hpp).
 #include "fas_cache_attn.hpp"
-#include "fas_launch.hpp"
+#include "fas_rows_launch.hpp"
 
 namespace fas {
 
 template <class E, int D, int BITS>
 static hipError_t attn_t(const RowsParams& p, hipStream_t s) {
-  const int rows = p.G * p.M;
-  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.nrb * p.nsplit)), block(256);
-  const dim3 merge((unsigned)((int64_t)p.B * p.Hk * rows));
-  if (rows <= kCacheFewRows) {
-    hipLaunchKernelGGL((cache_few_kernel<E, D, BITS>), grid, block, 0, s, p);
-    if (p.nsplit > 1)
-      hipLaunchKernelGGL((merge_kernel<E, D, kCacheFewRows, kCacheFewKeys>), merge, block, 0,
-                         s, p);
-  } else {
-    hipLaunchKernelGGL((rows_kernel<E, D, CacheSource<E, D, BITS>>), grid, block, 0, s, p);
-    if (p.nsplit > 1)
-      hipLaunchKernelGGL((merge_kernel<E, D, kRowsBlock, kRowsKeys>), merge, block,
-                         0, s, p);
-  }
-  return hipGetLastError();
+  return launch_rows<E, D, CacheFewSource<E, D, BITS>, CacheSource<E, D, BITS>>(p, s);
 }
 
 template <class E, int D>

@@ -325,9 +325,9 @@ namespace fas {
 // Most workgroups that share a row's keys (merge_kernel holds one part a
 // thread).
 constexpr int kRowsMaxSplits = 256;
-// Virtual rows of cache_few_kernel and of a rows_kernel block; their key tiles.
-constexpr int kCacheFewRows = 32, kRowsBlock = 128;
-constexpr int kCacheFewKeys = 32, kRowsKeys = 64;
+// Virtual rows of few_kernel and of a rows_kernel block; their key tiles.
+constexpr int kFewRows = 32, kRowsBlock = 128;
+constexpr int kFewKeys = 32, kRowsKeys = 64;
 
 // Attention with a window and sinks over dense keys or the quantised cache
 // (fas_rows.hpp).

@@ -13,6 +13,13 @@
 // virtual rows span 128 / G positions, and the window's tiles that only some of
 // them see are few.
 //
+//   few_kernel    at most 32 virtual rows (decoding).  Bound by the bytes of K
+//                 and V, so nothing is shared between the waves: each of the
+//                 four streams tiles of 32 keys of its own into registers, and
+//                 only V passes through a small LDS tile of the wave's, whose
+//                 transposing read gives the A operand of O^T += V^T P^T.  The
+//                 products are 16x16x32: one or two tiles of 16 rows, so that
+//                 few rows take few registers and more waves hide the latency.
 //   rows_kernel   128 virtual rows, four waves of 32, over key tiles of 64 that
 //                 they share through LDS.  How a tile gets there is the
 //                 source's business (dense rows by LDS DMA, codes through
@@ -56,7 +63,7 @@ __device__ __forceinline__ RowsPlan rows_plan(const RowsParams& p, int b, int rb
     c.tiles = c.sink_tiles + (c.hi + BN) / BN - c.win;
   }
   c.per = max(p.min_tiles, (c.tiles + p.nsplit - 1) / p.nsplit);
-  if (BM == 32) c.per = (c.per + 3) & ~3;  // the few-rows kernel's four waves take turns
+  if (BM == kFewRows) c.per = (c.per + 3) & ~3;  // few_kernel's four waves take turns
   c.used = max(1, (c.tiles + c.per - 1) / c.per);
   return c;
 }
@@ -125,28 +132,6 @@ struct SoftRows {
     }
     l += lt;
   }
-  // Adds another wave's rows (the same lanes hold the same rows).
-  __device__ __forceinline__ void save(float* a, int lane) const {
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) a[(16 * db + r) * 64 + lane] = o[db][r];
-    a[16 * DB * 64 + lane] = m;
-    a[(16 * DB + 1) * 64 + lane] = l;
-  }
-  __device__ __forceinline__ void add(const float* a, int lane, float qk) {
-    const float mo = a[16 * DB * 64 + lane], lo = a[(16 * DB + 1) * 64 + lane];
-    const float mn = fmaxf(m, mo);
-    const float a0 = m == neg_inf() ? 0.f : exp2f_fast((m - mn) * qk);
-    const float a1 = mo == neg_inf() ? 0.f : exp2f_fast((mo - mn) * qk);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] = o[db][r] * a0 + a[(16 * db + r) * 64 + lane] * a1;
-    l = l * a0 + lo * a1;
-    m = mn;
-  }
-  static constexpr int kSaved = (16 * DB + 2) * 64;  // floats
 };
 
 // NaN blocks: bit `group` of flag(row) says that the V block of tile row `row`
@@ -224,6 +209,279 @@ __device__ __forceinline__ u32x4 load_q(const RowsParams& p, int b, int hk, int 
   if (v >= p.G * p.M) return u32x4{0u, 0u, 0u, 0u};
   return *reinterpret_cast<const u32x4*>(p.q + b * p.sq0 + h * p.sq1 + (int64_t)i * p.sq2 + d0) ^
          p.qneg;
+}
+
+// ---------------------------------------------------------------- few rows
+
+__device__ __forceinline__ f32x4 mma16(F16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(BF16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// x combined over the four lanes that share a row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return xor32_max(x);
+}
+__device__ __forceinline__ float quad_add(float x) { return xor32_add(x + __shfl_xor(x, 16)); }
+
+// Byte offset of (row, 16-byte chunk) in a wave's 32 x D tile of values.  The
+// rows that a transposing read takes at once (8 rows, two chunks) fall on
+// different banks, and so do the rows that lanes write side by side.
+template <int D>
+__device__ __forceinline__ uint32_t few_off(int row, int chunk) {
+  constexpr int CH = D / 8, S = D == 128 ? 0 : D == 64 ? 1 : D == 32 ? 2 : 3;
+  return (uint32_t)(row * 2 * D + ((chunk ^ (2 * ((row >> S) & (CH / 2 - 1)))) << 4));
+}
+
+// Rows of few_kernel: lane (c, g), c = lane % 16, g = lane / 16, holds row 16 n + c
+// of column tile n; of its scores keys 16 t + 4 g + r, of O^T channels
+// 16 dt + 4 g + r.
+template <class E, int D, int NC>
+struct FewRows {
+  static constexpr int DT = D / 16;
+  float m[NC], l[NC];
+  f32x4 o[NC][DT];
+  __device__ __forceinline__ FewRows() {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      m[n] = neg_inf();
+      l[n] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[n][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // As SoftRows::weights and tile.
+  __device__ __forceinline__ float weights(int n, const f32x4 (&s)[2], float qk, u32x4& pb) {
+    const float nb = (m[n] == neg_inf() ? 0.f : m[n]) * qk;
+    float pv[8], lt = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pv[e] = exp2f_fast(fmaf(s[e >> 2][e & 3], qk, -nb));
+      lt += pv[e];
+    }
+    pb = u32x4{E::pack(pv[0], pv[1]), E::pack(pv[2], pv[3]), E::pack(pv[4], pv[5]),
+               E::pack(pv[6], pv[7])};
+    return lt;
+  }
+  __device__ __forceinline__ void tile(const f32x4 (&s)[NC][2], float qk, u32x4 (&pb)[NC]) {
+    float lt[NC];
+    bool redo = false;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      lt[n] = weights(n, s[n], qk, pb[n]);
+      redo = redo || !(lt[n] <= 16384.f) || m[n] == neg_inf();
+    }
+    if (__builtin_amdgcn_ballot_w64(redo) != 0) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        float mx = neg_inf();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[n][e >> 2][e & 3]);
+        mx = quad_max(mx);
+        if (mx > m[n] && (m[n] == neg_inf() || (mx - m[n]) * qk > 8.f)) {
+          const float a = m[n] == neg_inf() ? 0.f : exp2f_fast((m[n] - mx) * qk);
+          l[n] *= a;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[n][dt] *= a;
+          m[n] = mx;
+        }
+        lt[n] = weights(n, s[n], qk, pb[n]);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) l[n] += lt[n];
+  }
+  static constexpr int kSaved = NC * (4 * DT + 2) * 64;  // floats
+  __device__ __forceinline__ void save(float* a, int lane) const {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4*>(a + ((n * DT + dt) * 64 + lane) * 4) = o[n][dt];
+      a[(NC * DT * 4 + n) * 64 + lane] = m[n];
+      a[(NC * (DT * 4 + 1) + n) * 64 + lane] = l[n];
+    }
+  }
+  // Adds another wave's rows (the same lanes hold the same rows).
+  __device__ __forceinline__ void add(const float* a, int lane, float qk) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float mo = a[(NC * DT * 4 + n) * 64 + lane], lo = a[(NC * (DT * 4 + 1) + n) * 64 + lane];
+      const float mn = fmaxf(m[n], mo);
+      const float a0 = m[n] == neg_inf() ? 0.f : exp2f_fast((m[n] - mn) * qk);
+      const float a1 = mo == neg_inf() ? 0.f : exp2f_fast((mo - mn) * qk);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        o[n][dt] = o[n][dt] * a0 +
+                   *reinterpret_cast<const f32x4*>(a + ((n * DT + dt) * 64 + lane) * 4) * a1;
+      // (Without an offset a sum is 0, or NaN where the scores were.)
+      l[n] = (m[n] == neg_inf() ? l[n] : l[n] * a0) + (mo == neg_inf() ? lo : lo * a1);
+      m[n] = mn;
+    }
+  }
+};
+
+// SRC (a tile source): fetch(t) starts tile t's loads and take() makes it the
+// current one (kAhead: the loop fetches the next tile before it uses the
+// current one); key(i, m) is the A operand of keys 16 i .. and k-step m, whose
+// channels start at channel(m, g) in lane group g; values(put) hands the value
+// rows to put(row, chunk, 16 bytes).
+// Waves per SIMD (few_waves): as many as the registers of O^T and of the tiles
+// under way leave room for; left free, the compiler spreads over twice as many
+// registers.
+constexpr int few_waves(int d, int nc) { return d == 128 ? (nc == 1 ? 3 : 2) : nc == 1 ? 4 : 3; }
+template <class E, int D, int NC, class SRC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_waves(D, NC))))
+void few_kernel(const RowsParams p) {
+  constexpr int NW = 4, BN = kFewKeys, KS = D >= 32 ? D / 32 : 1, DT = D / 16;
+  using Rows = FewRows<E, D, NC>;
+  union Lds {
+    uint8_t v[NW][BN * 2 * D];
+    float rows[NW / 2][Rows::kSaved];
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int split = (int)(blockIdx.x % (uint32_t)p.nsplit), bhk = (int)(blockIdx.x / (uint32_t)p.nsplit);
+  const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
+  const RowsPlan plan = rows_plan<kFewRows, BN>(p, b, 0);
+  if (split >= plan.used) return;
+  const int t1 = min(plan.tiles, (split + 1) * plan.per);
+
+  // Rows that do not exist see what the last row sees; nothing of theirs is
+  // stored.
+  int pos[NC];
+  u32x4 q[NC][KS];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int v = 16 * n + c;
+    pos[n] = min(plan.pos0 + v / p.G, plan.hi);
+#pragma unroll
+    for (int m = 0; m < KS; ++m) {
+      q[n][m] = load_q<D>(p, b, hk, v, SRC::channel(m, g));
+      if (D < 32 && g >= 2) q[n][m] = u32x4{0u, 0u, 0u, 0u};  // half the contraction is padding
+    }
+  }
+
+  SRC src(p, plan, b, hk, lane);
+  Rows a;
+  uint8_t* vt = lds.v[wave];
+  // Transposing reads: lane j of a 16-lane group fetches 8 bytes of key 4 g + j / 4,
+  // channels 4 (j % 4) .., and receives channel j of keys 4 g .. 4 g + 3.
+  const int vkey = 4 * g + (c >> 2), vchunk = (c & 3) >> 1, vsub = 8 * (c & 1);
+  int t = split * plan.per + wave;
+  if (SRC::kAhead && t < t1) src.fetch(t);
+  for (; t < t1; t += NW) {
+    const int k0 = plan.tile(t) * BN;
+    if constexpr (!SRC::kAhead) src.fetch(t);
+    src.take();
+    if (SRC::kAhead && t + NW < t1) src.fetch(t + NW);
+    f32x4 s[NC][2];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < KS; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4 k = src.key(i, m);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][i] = mma16(E{}, k, q[n][m], s[n][i]);
+      }
+    if (!rows_full(p, plan, k0, BN)) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!row_sees(p, pos[n], k0 + 16 * (e >> 2) + 4 * g + (e & 3)))
+            s[n][e >> 2][e & 3] = neg_inf();
+    }
+    // A wave's LDS accesses run in issue order: only the compiler must keep the
+    // last tile's reads, these writes and the reads below in theirs.
+    __builtin_amdgcn_wave_barrier();
+    src.values([&](int row, int chunk, u32x4 x) __attribute__((always_inline)) {
+      *reinterpret_cast<u32x4*>(vt + few_off<D>(row, chunk)) = x;
+    });
+    u32x4 pb[NC];
+    a.tile(s, p.qk_scale, pb);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      // Contraction index 8 g + e is key 4 g + e, or 16 + 4 g + e - 4: the order
+      // of the weights.
+      const fp16x4_lds r0 = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+          (FAS_LDS fp16x4_lds*)(vt + few_off<D>(vkey, 2 * dt + vchunk) + vsub));
+      const fp16x4_lds r1 = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+          (FAS_LDS fp16x4_lds*)(vt + few_off<D>(vkey + 16, 2 * dt + vchunk) + vsub));
+      const u32x2 x = __builtin_bit_cast(u32x2, r0), y = __builtin_bit_cast(u32x2, r1);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) a.o[n][dt] = mma16(E{}, u32x4{x.x, x.y, y.x, y.y}, pb[n], a.o[n][dt]);
+    }
+    if constexpr (SRC::kNanBlocks) {
+      const uint32_t nan = src.nan();
+      if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+        for (int row = 0; row < BN; ++row) {
+          const uint32_t f = SRC::nan_row(nan, row);
+          if (f == 0) continue;
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            const bool sees = row_sees(p, pos[n], k0 + row);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+              if ((f >> (dt / 2)) & 1u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  a.o[n][dt][r] = sees ? __builtin_nanf("") : a.o[n][dt][r];
+          }
+        }
+      }
+    }
+  }
+  // The four waves' rows, pairwise.
+  __syncthreads();
+  if (wave >= 2) a.save(lds.rows[wave - 2], lane);
+  __syncthreads();
+  if (wave < 2) a.add(lds.rows[wave], lane, p.qk_scale);
+  __syncthreads();
+  if (wave == 1) a.save(lds.rows[0], lane);
+  __syncthreads();
+  if (wave != 0) return;
+  a.add(lds.rows[0], lane, p.qk_scale);
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int v = 16 * n + c;
+    const float l = quad_add(a.l[n]);
+    if (v >= p.G * p.M) continue;
+    const int i = v / p.G, h = hk * p.G + (v - i * p.G);
+    const bool live = i < plan.cnt;
+    if (plan.used > 1) {
+      const int64_t row = ((int64_t)bhk * p.nsplit + split) * p.Rpad + v;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4*>(p.part_o + row * D + 16 * dt + 4 * g) = a.o[n][dt];
+      if (g == 0)
+        *reinterpret_cast<f32x2*>(p.part_ml + 2 * row) =
+            f32x2{a.m[n] == neg_inf() ? neg_inf() : a.m[n] * p.qk_scale, l};
+      continue;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* out = p.o + b * p.so0 + h * p.so1 + (int64_t)i * p.so2;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const f32x4 o = a.o[n][dt] * inv;
+      *reinterpret_cast<u32x2*>(out + 16 * dt + 4 * g) =
+          live ? u32x2{E::pack(o[0], o[1]), E::pack(o[2], o[3])} : u32x2{0u, 0u};
+    }
+    if (g == 0 && p.lse != nullptr)
+      p.lse[b * p.sl0 + h * p.sl1 + (int64_t)i * p.sl2] =
+          !live || l == 0.f ? neg_inf()
+                            : (a.m[n] * p.qk_scale + log2f_fast(l)) * 0.69314718055994531f;
+  }
 }
 
 // ---------------------------------------------------------------- many rows

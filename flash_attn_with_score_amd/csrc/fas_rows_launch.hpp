@@ -1,0 +1,29 @@
+// Launch of a call's rows (fas_rows.hpp), whatever its tile sources: at most 16
+// virtual rows, at most 32, or more, and the merge of split rows.
+#pragma once
+#include "fas_launch.hpp"
+#include "fas_rows.hpp"
+
+namespace fas {
+
+template <class E, int D, class FEW, class MANY>
+hipError_t launch_rows(const RowsParams& p, hipStream_t s) {
+  const int rows = p.G * p.M;
+  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.nrb * p.nsplit)), block(256);
+  if (rows <= 16)
+    hipLaunchKernelGGL((few_kernel<E, D, 1, FEW>), grid, block, 0, s, p);
+  else if (rows <= kFewRows)
+    hipLaunchKernelGGL((few_kernel<E, D, 2, FEW>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((rows_kernel<E, D, MANY>), grid, block, 0, s, p);
+  if (p.nsplit > 1) {
+    const dim3 merge((unsigned)((int64_t)p.B * p.Hk * rows));
+    if (rows <= kFewRows)
+      hipLaunchKernelGGL((merge_kernel<E, D, kFewRows, kFewKeys>), merge, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((merge_kernel<E, D, kRowsBlock, kRowsKeys>), merge, block, 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace fas

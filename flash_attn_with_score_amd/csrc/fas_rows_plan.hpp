@@ -16,11 +16,11 @@ struct RowsSplit {
 };
 
 // rows: virtual rows of each of `groups` (batch entry, KV head) pairs; keys:
-// the most that a sequence can hold; few: cache_few_kernel runs.
+// the most that a sequence can hold; few: few_kernel runs.
 inline RowsSplit rows_split(int64_t groups, int64_t rows, int64_t tokens, int64_t keys,
                             int64_t window, int64_t sinks, int64_t D, bool few) {
   RowsSplit w{};
-  const int64_t bm = few ? kCacheFewRows : kRowsBlock, bn = few ? kCacheFewKeys : kRowsKeys;
+  const int64_t bm = few ? kFewRows : kRowsBlock, bn = few ? kFewKeys : kRowsKeys;
   w.nrb = (rows + bm - 1) / bm;
   w.rpad = w.nrb * bm;
   // Key tiles that a row block can need, whatever the sequences' lengths.

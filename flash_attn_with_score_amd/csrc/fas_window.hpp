@@ -1,5 +1,5 @@
-// gfx950 windowed attention over dense keys, forward (rows_kernel of
-// fas_rows.hpp with DenseSource) and backward.
+// gfx950 windowed attention over dense keys, forward (rows_kernel and few_kernel
+// of fas_rows.hpp with DenseSource and DenseFewSource) and backward.
 //
 // Query row i is at position p = (N - M) + i and sees key j iff j <= p and
 // (j > p - window or j < sinks).  The backward has attention()'s three passes
@@ -61,6 +61,49 @@ struct DenseSource {
   __device__ __forceinline__ void land(int) { vm_wait_all(); }
   __device__ __forceinline__ const uint16_t* keys(int stage) const { return lds.kv[stage][0]; }
   __device__ __forceinline__ const uint16_t* values(int stage) const { return lds.kv[stage][1]; }
+};
+
+// Tiles of 32 dense rows for few_kernel, in registers.  (No tile ahead: a
+// tile of 32 keys takes 64 registers at D = 128, and the other waves' loads
+// cover the wait.)
+template <class E, int D>
+struct DenseFewSource {
+  static constexpr bool kAhead = false, kNanBlocks = false;
+  static constexpr int KS = D >= 32 ? D / 32 : 1, VL = D / 16;
+  u32x4 k[2][KS], v[VL];
+  const RowsPlan& plan;
+  const uint8_t *kp, *vp;
+  const int64_t sk, sv;
+  const int c, lane;
+  __device__ __forceinline__ DenseFewSource(const RowsParams& p, const RowsPlan& plan_, int b,
+                                            int hk, int lane_)
+      : plan(plan_), kp(p.k + b * p.sk0 + hk * p.sk1 + 2 * channel(0, lane_ >> 4)),
+        vp(p.v + b * p.sv0 + hk * p.sv1 + 16 * (lane_ % (D / 8))), sk(p.sk2), sv(p.sv2),
+        c(lane_ & 15), lane(lane_) {}
+  static __device__ __forceinline__ int channel(int m, int g) {
+    return D >= 32 ? 32 * m + 8 * g : 8 * (g & 1);
+  }
+  __device__ __forceinline__ void fetch(int t) {
+    const int k0 = plan.tile(t) * kFewKeys;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* row = kp + (int64_t)min(k0 + 16 * i + c, plan.len - 1) * sk;
+#pragma unroll
+      for (int m = 0; m < KS; ++m) k[i][m] = *reinterpret_cast<const u32x4*>(row + 64 * m);
+    }
+#pragma unroll
+    for (int j = 0; j < VL; ++j)
+      v[j] = *reinterpret_cast<const u32x4*>(
+          vp + (int64_t)min(k0 + value_row(j), plan.len - 1) * sv);
+  }
+  __device__ __forceinline__ int value_row(int j) const { return (64 * j + lane) / (D / 8); }
+  __device__ __forceinline__ void take() {}
+  __device__ __forceinline__ u32x4 key(int i, int m) const { return k[i][m]; }
+  template <class PUT>
+  __device__ __forceinline__ void values(PUT&& put) const {
+#pragma unroll
+    for (int j = 0; j < VL; ++j) put(value_row(j), lane % (D / 8), v[j]);
+  }
 };
 
 // Part of the fp32 workspace that piece `piece` of key block kb writes.

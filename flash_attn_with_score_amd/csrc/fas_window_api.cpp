@@ -40,8 +40,9 @@ int check_window(const char* fn, const fas_attn_args* a, int64_t window, int64_t
 }
 
 fas::RowsSplit fwd_split(const Problem& pr, int64_t window, int64_t sinks) {
-  return fas::rows_split((int64_t)pr.B * pr.Hk, (int64_t)pr.G * pr.M, pr.M, pr.N, window, sinks, pr.D,
-                         false);
+  const int64_t rows = (int64_t)pr.G * pr.M;
+  return fas::rows_split((int64_t)pr.B * pr.Hk, rows, pr.M, pr.N, window, sinks, pr.D,
+                         rows <= fas::kFewRows);
 }
 
 // Workgroups per key block of the dK/dV kernel, and its workspace.  A block

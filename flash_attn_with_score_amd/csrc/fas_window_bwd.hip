@@ -1,19 +1,8 @@
-// Instances and launchers of the windowed attention (fas_window.hpp).
+// Instances and launcher of the windowed attention's backward (fas_window.hpp).
 #include "fas_launch.hpp"
 #include "fas_window.hpp"
 
 namespace fas {
-
-template <class E, int D>
-static hipError_t fwd_t(const RowsParams& p, hipStream_t s) {
-  const dim3 block(256);
-  hipLaunchKernelGGL((rows_kernel<E, D, DenseSource<E, D>>),
-                     dim3((unsigned)((int64_t)p.B * p.Hk * p.nrb * p.nsplit)), block, 0, s, p);
-  if (p.nsplit > 1)
-    hipLaunchKernelGGL((merge_kernel<E, D, kRowsBlock, kRowsKeys>),
-                       dim3((unsigned)((int64_t)p.B * p.H * p.M)), block, 0, s, p);
-  return hipGetLastError();
-}
 
 template <class E, int D>
 static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
@@ -41,16 +30,6 @@ static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
 }
 
 template <class E>
-static hipError_t fwd_d(const RowsParams& p, int d, hipStream_t s) {
-  switch (d) {
-    case 16: return fwd_t<E, 16>(p, s);
-    case 32: return fwd_t<E, 32>(p, s);
-    case 64: return fwd_t<E, 64>(p, s);
-    case 128: return fwd_t<E, 128>(p, s);
-  }
-  return hipErrorInvalidValue;
-}
-template <class E>
 static hipError_t bwd_d(const WindowBwdParams& p, int d, hipStream_t s) {
   switch (d) {
     case 16: return bwd_t<E, 16>(p, s);
@@ -61,9 +40,6 @@ static hipError_t bwd_d(const WindowBwdParams& p, int d, hipStream_t s) {
   return hipErrorInvalidValue;
 }
 
-hipError_t launch_window_fwd(const RowsParams& p, int dtype, int d, hipStream_t s) {
-  return dtype == 0 ? fwd_d<F16>(p, d, s) : fwd_d<BF16>(p, d, s);
-}
 hipError_t launch_window_bwd(const WindowBwdParams& p, int dtype, int d, hipStream_t s) {
   return dtype == 0 ? bwd_d<F16>(p, d, s) : bwd_d<BF16>(p, d, s);
 }

@@ -57,24 +57,26 @@ def _check_capture(ctx, device) -> None:
                 "graph of the same leaves lives; drop its outputs before the capture")
 
 
+def _forward(q, k, v, window, sinks, sm_scale, want_lse):
+    p = _common.finish_problem(q, k, v, sm_scale)
+    o = _common.new_output(p.q)
+    L = torch.empty((p.B, p.H, p.M), device=q.device, dtype=torch.float32) if want_lse else None
+    args = _native.pack_args(p.q, p.k, p.v, o, True, p.sm_scale)
+    ws_ptr, ws_bytes, ws = _workspace(args, window, sinks, 0, q.device)
+    _common.call("fas_attention_window", p.q, args, window, sinks,
+                 0 if L is None else L.data_ptr(), None if L is None else _native.pack_strides(L),
+                 ws_ptr, ws_bytes)
+    return p, o, L
+
+
 class WindowAttention(torch.autograd.Function):
     """fas_attention_window and fas_attention_window_backward."""
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, sm_scale, return_log_normalizer):
-        p = _common.finish_problem(q, k, v, sm_scale)
-        o = _common.new_output(p.q)
-        need_grad = any(ctx.needs_input_grad[:3])
-        L = torch.empty((p.B, p.H, p.M), device=q.device, dtype=torch.float32) \
-            if need_grad or return_log_normalizer else None
-        args = _native.pack_args(p.q, p.k, p.v, o, True, p.sm_scale)
-        ws_ptr, ws_bytes, ws = _workspace(args, window, sinks, 0, q.device)
-        _common.call("fas_attention_window", p.q, args, window, sinks,
-                     0 if L is None else L.data_ptr(),
-                     None if L is None else _native.pack_strides(L), ws_ptr, ws_bytes)
-        if need_grad:
-            ctx.save_for_backward(p.q, p.k, p.v, o, L)
-            ctx.window, ctx.sinks, ctx.sm_scale = window, sinks, p.sm_scale
+        p, o, L = _forward(q, k, v, window, sinks, sm_scale, True)
+        ctx.save_for_backward(p.q, p.k, p.v, o, L)
+        ctx.window, ctx.sinks, ctx.sm_scale = window, sinks, p.sm_scale
         if return_log_normalizer:
             ctx.mark_non_differentiable(L)
             return o, L
@@ -111,9 +113,10 @@ def attention_window(q, k, v, window: int, sinks: int = 0, sm_scale: float | Non
         raise ValueError(f"flash_attn_with_score_amd: window {window} must be at least 1")
     if sinks < 0:
         raise ValueError(f"flash_attn_with_score_amd: sinks {sinks} must not be negative")
-    res = WindowAttention.apply(q, k, v, min(int(window), _MOST), min(int(sinks), _MOST), sm_scale,
-                                return_log_normalizer)
-    out = res[0] if return_log_normalizer else res
-    if out.grad_fn is not None:
-        _mark_leaves(out)
+    window, sinks = min(int(window), _MOST), min(int(sinks), _MOST)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        _, out, L = _forward(q, k, v, window, sinks, sm_scale, return_log_normalizer)
+        return (out, L) if return_log_normalizer else out
+    res = WindowAttention.apply(q, k, v, window, sinks, sm_scale, return_log_normalizer)
+    _mark_leaves(res[0] if return_log_normalizer else res)
     return res
