@@ -147,9 +147,9 @@ int check_attn(const char* fn, const fas_kv_cache* c, const fas_kv_query* a) {
 
 fas::RowsSplit attn_split(const fas_kv_cache* c, const fas_kv_query* a) {
   const int64_t rows = a->heads_q / c->heads * a->tokens;
-  return fas::rows_split(c->batch * c->heads, rows, a->tokens,
+  return fas::rows_split(c->batch, c->batch * c->heads, rows, a->tokens,
                          a->lengths == nullptr ? a->lengths_all : c->capacity, a->window, a->sinks,
-                         c->head_dim, rows <= fas::kFewRows);
+                         c->head_dim, rows <= fas::kFewRows, a->lengths != nullptr);
 }
 
 }  // namespace
@@ -193,7 +193,7 @@ int fas_attention_kv_cache(const fas_kv_cache* c, const fas_kv_query* a, float* 
   }
   const fas::RowsSplit w = attn_split(c, a);
   if ((rc = fas::check_rows_workspace(fn, w.total, ws, ws_bytes))) return rc;
-  if (c->batch * c->heads * w.nrb * w.nsplit > INT_MAX)
+  if (w.grid > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more row blocks than one launch takes");
   fas::RowsParams p{};
   p.q = static_cast<const uint16_t*>(a->q);

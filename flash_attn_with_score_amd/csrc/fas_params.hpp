@@ -351,12 +351,17 @@ struct RowsParams {
   int nrb;                 // blocks of virtual rows
   int nsplit;              // workgroups per row block, at most kRowsMaxSplits
   int min_tiles;           // least key tiles of a workgroup
+  int balance, slots;      // few rows: the batch's tiles over `slots` workgroups
+  int grid;                // workgroups launched
+  int* part_per;           // balance: tiles of a workgroup, for merge_kernel
   int Rpad;                // virtual rows, padded to whole blocks
   float* part_o;           // (B * Hk, nsplit, Rpad, D): unnormalised O
   float* part_ml;          // (B * Hk, nsplit, Rpad, 2): base-2 exponent offset, sum of weights
   float qk_scale;          // |sm_scale| * log2(e)
   uint32_t qneg;           // 0x80008000 to negate q (negative sm_scale), else 0
 };
+// Sequences that few_kernel balances (one a lane).
+constexpr int kBalanceBatch = 64;
 // Window of a call without one; pos - window stays inside 32 bits.
 constexpr int kNoWindow = 1 << 30;
 

@@ -47,8 +47,9 @@ struct RowsPlan {
     return i < sink_tiles ? i : i - sink_tiles + win;
   }
 };
+// Sequence b's block rb of the plan, but for how its tiles are dealt.
 template <int BM, int BN>
-__device__ __forceinline__ RowsPlan rows_plan(const RowsParams& p, int b, int rb) {
+__device__ __forceinline__ RowsPlan rows_tiles(const RowsParams& p, int b, int rb) {
   RowsPlan c;
   c.len = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.capacity) : p.lengths_all;
   c.cnt = p.counts != nullptr ? min(max(p.counts[b], 0), p.M) : p.M;
@@ -62,9 +63,73 @@ __device__ __forceinline__ RowsPlan rows_plan(const RowsParams& p, int b, int rb
     c.sink_tiles = min(c.win, (min(p.sinks, c.hi + 1) + BN - 1) / BN);
     c.tiles = c.sink_tiles + (c.hi + BN) / BN - c.win;
   }
+  return c;
+}
+// How the tiles of one block are dealt: evenly, to at most nsplit workgroups.
+template <int BM, int BN>
+__device__ __forceinline__ RowsPlan rows_plan(const RowsParams& p, int b, int rb) {
+  RowsPlan c = rows_tiles<BM, BN>(p, b, rb);
   c.per = max(p.min_tiles, (c.tiles + p.nsplit - 1) / p.nsplit);
   if (BM == kFewRows) c.per = (c.per + 3) & ~3;  // few_kernel's four waves take turns
   c.used = max(1, (c.tiles + c.per - 1) / c.per);
+  return c;
+}
+
+// Inclusive scans over the wave's lanes, as six lane shifts of the vector ALU.
+template <class F>
+__device__ __forceinline__ int wave_scan(int v, F&& f) {
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));  // row_shr:2
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));  // row_shr:4
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));  // row_shr:8
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return v;
+}
+
+// Few rows of a batch whose lengths the host does not know (balance: at most
+// kBalanceBatch sequences): all take workgroups of about the same length, the
+// batch's tiles over about p.slots of them, and the workgroups that have work
+// come first in the grid.  Lane i works out sequence i.  Dealt evenly instead, a
+// ragged batch waits for its longest sequence.  Returns the workgroup's plan
+// and where it stands (split < 0: no work).
+template <int BN>
+__device__ __forceinline__ RowsPlan rows_balanced(const RowsParams& p, int id, int& b, int& hk,
+                                                  int& split) {
+  const int lane = (int)threadIdx.x & 63;
+  RowsPlan c = rows_tiles<kFewRows, BN>(p, min(lane, p.B - 1), 0);
+  const bool mine = lane < p.B;
+  const int tiles = mine ? c.tiles : 0;
+  auto sum = [](int x) {
+    return __builtin_amdgcn_readlane(wave_scan(x, [](int a, int b) { return a + b; }), 63);
+  };
+  const int64_t total = sum(tiles);
+  const int most =
+      __builtin_amdgcn_readlane(wave_scan(tiles, [](int x, int y) { return max(x, y); }), 63);
+  const int least = max(p.min_tiles, (most + p.nsplit - 1) / p.nsplit);
+  int per = (max(least, (int)((total * p.Hk + p.slots - 1) / p.slots)) + 3) & ~3;
+  // The sequences' last workgroups are parts of one, half of one in the mean:
+  // longer ones until the batch fits the slots, or nearly.
+  int used = 0;
+#pragma unroll
+  for (int it = 0; it < 3; ++it) {
+    used = mine ? max(1, (tiles + per - 1) / per) : 0;
+    const int over = sum(used) * p.Hk - p.slots;
+    if (it == 2 || over <= 0) break;
+    per = (per + (int)(((int64_t)per * over + p.slots - 1) / p.slots) + 3) & ~3;
+  }
+  const int end = wave_scan(used, [](int x, int y) { return x + y; }) * p.Hk;
+  b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine && end <= id));
+  split = -1;
+  if (b < p.B) {
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
+    c = RowsPlan{of(c.len), of(c.cnt), of(c.pos0), of(c.lo), of(c.hi), of(c.sink_tiles), of(c.win),
+                 of(c.tiles), per, of(used)};
+    const int rest = id - (of(end) - c.used * p.Hk);
+    hk = __builtin_amdgcn_readfirstlane(rest / c.used);
+    split = rest - hk * c.used;
+    if (id == 0 && threadIdx.x == 0) *p.part_per = per;
+  }
   return c;
 }
 
@@ -348,10 +413,20 @@ void few_kernel(const RowsParams p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-  const int split = (int)(blockIdx.x % (uint32_t)p.nsplit), bhk = (int)(blockIdx.x / (uint32_t)p.nsplit);
-  const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  const RowsPlan plan = rows_plan<kFewRows, BN>(p, b, 0);
-  if (split >= plan.used) return;
+  int split, b, hk;
+  RowsPlan plan;
+  if (p.balance) {
+    plan = rows_balanced<BN>(p, (int)blockIdx.x, b, hk, split);
+    if (split < 0) return;
+  } else {
+    split = (int)(blockIdx.x % (uint32_t)p.nsplit);
+    const int bhk = (int)(blockIdx.x / (uint32_t)p.nsplit);
+    b = bhk / p.Hk;
+    hk = bhk - b * p.Hk;
+    plan = rows_plan<kFewRows, BN>(p, b, 0);
+    if (split >= plan.used) return;
+  }
+  const int bhk = b * p.Hk + hk;
   const int t1 = min(plan.tiles, (split + 1) * plan.per);
 
   // Rows that do not exist see what the last row sees; nothing of theirs is
@@ -590,7 +665,11 @@ __global__ __launch_bounds__(256) void merge_kernel(const RowsParams p) {
   const int rows = p.G * p.M;
   const int bhk = (int)(blockIdx.x / (uint32_t)rows), v = (int)(blockIdx.x - (uint32_t)bhk * (uint32_t)rows);
   const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  const RowsPlan plan = rows_plan<BM, BN>(p, b, v / BM);
+  RowsPlan plan = rows_plan<BM, BN>(p, b, v / BM);
+  if (BM == kFewRows && p.balance) {
+    plan.per = *p.part_per;
+    plan.used = max(1, (plan.tiles + plan.per - 1) / plan.per);
+  }
   if (plan.used == 1) return;
   const int64_t row0 = (int64_t)bhk * p.nsplit * p.Rpad + v;
   static_assert(kRowsMaxSplits == 256, "one part a thread");

@@ -9,7 +9,7 @@ namespace fas {
 template <class E, int D, class FEW, class MANY>
 hipError_t launch_rows(const RowsParams& p, hipStream_t s) {
   const int rows = p.G * p.M;
-  const dim3 grid((unsigned)((int64_t)p.B * p.Hk * p.nrb * p.nsplit)), block(256);
+  const dim3 grid((unsigned)p.grid), block(256);
   if (rows <= 16)
     hipLaunchKernelGGL((few_kernel<E, D, 1, FEW>), grid, block, 0, s, p);
   else if (rows <= kFewRows)

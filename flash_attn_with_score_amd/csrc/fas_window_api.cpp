@@ -41,8 +41,8 @@ int check_window(const char* fn, const fas_attn_args* a, int64_t window, int64_t
 
 fas::RowsSplit fwd_split(const Problem& pr, int64_t window, int64_t sinks) {
   const int64_t rows = (int64_t)pr.G * pr.M;
-  return fas::rows_split((int64_t)pr.B * pr.Hk, rows, pr.M, pr.N, window, sinks, pr.D,
-                         rows <= fas::kFewRows);
+  return fas::rows_split(pr.B, (int64_t)pr.B * pr.Hk, rows, pr.M, pr.N, window, sinks, pr.D,
+                         rows <= fas::kFewRows, false);
 }
 
 // Workgroups per key block of the dK/dV kernel, and its workspace.  A block
@@ -107,7 +107,7 @@ int fas_attention_window(const fas_attn_args* a, int64_t window, int64_t sinks, 
   }
   const fas::RowsSplit w = fwd_split(pr, window, sinks);
   if ((rc = fas::check_rows_workspace(fn, w.total, ws, ws_bytes))) return rc;
-  if ((int64_t)pr.B * pr.Hk * w.nrb * w.nsplit > INT_MAX)
+  if (w.grid > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more row blocks than one launch takes");
   fas::RowsParams p{};
   p.q = static_cast<const uint16_t*>(a->q);
