@@ -63,16 +63,15 @@ struct CacheFewSource {
     }
   }
   __device__ __forceinline__ void fetch(int t) {
-    const int k0 = plan.tile(t) * kFewKeys;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t r = min(k0 + 16 * i + c, plan.len - 1);
+      const int64_t r = plan.row(t * kFewKeys + 16 * i + c);
       words(next.kw[i], kc + r * skc);
       next.ks[i] = ks[r * sks];
     }
 #pragma unroll
     for (int i = 0; i < VR; ++i) {
-      const int64_t r = min(k0 + 16 * i + vrow, plan.len - 1);
+      const int64_t r = plan.row(t * kFewKeys + 16 * i + vrow);
       words(next.vw[i], vc + r * svc);
       next.vs[i] = vs[r * svs];
     }
@@ -164,7 +163,7 @@ struct CacheSource {
   }
   __device__ __forceinline__ void fetch(int t, int) {
     if (!stager) return;
-    const int64_t r = min(plan.tile(t) * kRowsKeys + row, plan.len - 1);
+    const int64_t r = plan.row(t * kRowsKeys + row);
     words(kw, kc + r * skc);
     words(vw, vc + r * svc);
     ksb = ks[r * sks];

@@ -454,4 +454,20 @@ __device__ __forceinline__ u32x4 lds_row_chunk(const uint16_t* tile, uint32_t of
 }
 __device__ __forceinline__ void opaque(uint32_t& o) { asm volatile("" : "+v"(o)); }
 
+// Schedule of one S^T = K Q^T tile (2 MFMAs and 2 operand fetches per
+// k-step): fetches run PD k-steps ahead of their MFMAs; NST global stores
+// of the same region go one per k-step.
+template <int KS, int NST>
+__device__ __forceinline__ void sched_score_tile() {
+  constexpr int PD = KS < 2 ? KS : 2;
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * PD, 0);  // DS read
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
+    if (i + PD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    if (i < NST) __builtin_amdgcn_sched_group_barrier(0x040, 1, 0);  // VMEM write
+  }
+  if (NST > KS) __builtin_amdgcn_sched_group_barrier(0x040, NST > KS ? NST - KS : 1, 0);
+}
+
 }  // namespace fas

@@ -220,22 +220,6 @@ __device__ __forceinline__ void interleave_mfma_stores() {
   }
 }
 
-// Schedule of one S^T = K Q^T tile (2 MFMAs and 2 operand fetches per
-// k-step): fetches run PD k-steps ahead of their MFMAs; NST global stores
-// of the same region go one per k-step.
-template <int KS, int NST>
-__device__ __forceinline__ void sched_score_tile() {
-  constexpr int PD = KS < 2 ? KS : 2;
-  __builtin_amdgcn_sched_group_barrier(0x100, 2 * PD, 0);  // DS read
-#pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
-    if (i + PD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    if (i < NST) __builtin_amdgcn_sched_group_barrier(0x040, 1, 0);  // VMEM write
-  }
-  if (NST > KS) __builtin_amdgcn_sched_group_barrier(0x040, NST > KS ? NST - KS : 1, 0);
-}
-
 // LDS of the region mode's row-major staging (kFwdRegion only: other
 // instances never instantiate these, so their LDS holds none of it).
 template <int NW>

@@ -36,16 +36,20 @@
 
 namespace fas {
 
-// Tiles of BN keys that a block of virtual rows [row0, row0 + BM) reads:
-// the first `sink_tiles` tiles of the cache, then `tiles - sink_tiles` tiles
-// from tile `win` on, dealt to `used` workgroups in runs of `per`.
+// The keys that a block of virtual rows [row0, row0 + BM) reads, as a list: the
+// first `ns` keys of the sequence (sinks in front of the window), then the keys
+// from the first row's window on.  Tile i is entries [BN i, BN i + BN) of the
+// list, so the sinks and the window's edge take no tiles of their own.  The tiles
+// are dealt to `used` workgroups in runs of `per`.
 struct RowsPlan {
   int len, cnt, pos0;  // keys, query rows, position of row 0
   int lo, hi;          // least and greatest position of the block's live rows (hi < lo: none)
-  int sink_tiles, win, tiles, per, used;
-  __device__ __forceinline__ int tile(int i) const {
-    return i < sink_tiles ? i : i - sink_tiles + win;
-  }
+  int ns, shift;       // entry e is key e, or e + shift from entry ns on
+  int tiles, per, used;
+  __device__ __forceinline__ int key(int e) const { return e < ns ? e : e + shift; }
+  // The key whose row stands in for entry e in memory: entries behind the
+  // last key take its row, their weight is 0.
+  __device__ __forceinline__ int row(int e) const { return min(key(e), len - 1); }
 };
 // Sequence b's block rb of the plan, but for how its tiles are dealt.
 template <int BM, int BN>
@@ -57,11 +61,12 @@ __device__ __forceinline__ RowsPlan rows_tiles(const RowsParams& p, int b, int r
   const int i0 = rb * BM / p.G, i1 = min(c.cnt, (rb * BM + BM - 1) / p.G + 1);  // rows [i0, i1)
   c.lo = c.pos0 + i0;
   c.hi = i1 > i0 ? c.pos0 + i1 - 1 : c.lo - 1;
-  c.sink_tiles = c.win = c.tiles = 0;
+  c.ns = c.shift = c.tiles = 0;
   if (c.hi >= max(c.lo, 0)) {
-    c.win = max(0, max(c.lo, 0) - p.window + 1) / BN;
-    c.sink_tiles = min(c.win, (min(p.sinks, c.hi + 1) + BN - 1) / BN);
-    c.tiles = c.sink_tiles + (c.hi + BN) / BN - c.win;
+    const int first = max(0, max(c.lo, 0) - p.window + 1);
+    c.ns = min(first, p.sinks);
+    c.shift = first - c.ns;
+    c.tiles = (c.hi + 1 - c.shift + BN - 1) / BN;
   }
   return c;
 }
@@ -123,7 +128,7 @@ __device__ __forceinline__ RowsPlan rows_balanced(const RowsParams& p, int id, i
   split = -1;
   if (b < p.B) {
     auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
-    c = RowsPlan{of(c.len), of(c.cnt), of(c.pos0), of(c.lo), of(c.hi), of(c.sink_tiles), of(c.win),
+    c = RowsPlan{of(c.len), of(c.cnt), of(c.pos0), of(c.lo), of(c.hi), of(c.ns), of(c.shift),
                  of(c.tiles), per, of(used)};
     const int rest = id - (of(end) - c.used * p.Hk);
     hk = __builtin_amdgcn_readfirstlane(rest / c.used);
@@ -133,10 +138,11 @@ __device__ __forceinline__ RowsPlan rows_balanced(const RowsParams& p, int id, i
   return c;
 }
 
-// Whether every live row of the block sees all keys [k0, k0 + n).
-__device__ __forceinline__ bool rows_full(const RowsParams& p, const RowsPlan& c, int k0,
-                                           int n) {
-  return k0 + n - 1 <= c.lo && (k0 > c.hi - p.window || k0 + n <= p.sinks);
+// Whether rows at positions [lo, hi] all see entries [e0, e0 + n).
+__device__ __forceinline__ bool rows_full(const RowsParams& p, const RowsPlan& c, int lo, int hi,
+                                          int e0, int n) {
+  return c.key(e0 + n - 1) <= lo &&
+         (e0 + n <= c.ns || max(e0, c.ns) + c.shift > hi - p.window || c.key(e0 + n - 1) < p.sinks);
 }
 __device__ __forceinline__ bool row_sees(const RowsParams& p, int pos, int key) {
   return key <= pos && (key > pos - p.window || key < p.sinks);
@@ -203,10 +209,10 @@ struct SoftRows {
 // reads as NaN; rows that see the key are set to NaN there.
 template <class E, int D, int NB, class F>
 __device__ __forceinline__ void set_nan_rows(SoftRows<E, D, NB>& a, const RowsParams& p,
-                                              int pos, int k0, F&& flag) {
+                                              const RowsPlan& plan, int pos, int e0, F&& flag) {
   for (int row = 0; row < 32 * NB; ++row) {
     const uint32_t f = flag(row);
-    const bool sees = row_sees(p, pos, k0 + row);
+    const bool sees = row_sees(p, pos, plan.key(e0 + row));
 #pragma unroll
     for (int db = 0; db < SoftRows<E, D, NB>::DB; ++db)
       if ((f >> db) & 1u)
@@ -453,7 +459,7 @@ void few_kernel(const RowsParams p) {
   int t = split * plan.per + wave;
   if (SRC::kAhead && t < t1) src.fetch(t);
   for (; t < t1; t += NW) {
-    const int k0 = plan.tile(t) * BN;
+    const int e0 = t * BN;
     if constexpr (!SRC::kAhead) src.fetch(t);
     src.take();
     if (SRC::kAhead && t + NW < t1) src.fetch(t + NW);
@@ -468,12 +474,12 @@ void few_kernel(const RowsParams p) {
 #pragma unroll
         for (int n = 0; n < NC; ++n) s[n][i] = mma16(E{}, k, q[n][m], s[n][i]);
       }
-    if (!rows_full(p, plan, k0, BN)) {
+    if (!rows_full(p, plan, plan.lo, plan.hi, e0, BN)) {
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (!row_sees(p, pos[n], k0 + 16 * (e >> 2) + 4 * g + (e & 3)))
+          if (!row_sees(p, pos[n], plan.key(e0 + 16 * (e >> 2) + 4 * g + (e & 3))))
             s[n][e >> 2][e & 3] = neg_inf();
     }
     // A wave's LDS accesses run in issue order: only the compiler must keep the
@@ -505,7 +511,7 @@ void few_kernel(const RowsParams p) {
           if (f == 0) continue;
 #pragma unroll
           for (int n = 0; n < NC; ++n) {
-            const bool sees = row_sees(p, pos[n], k0 + row);
+            const bool sees = row_sees(p, pos[n], plan.key(e0 + row));
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
               if ((f >> (dt / 2)) & 1u)
@@ -607,9 +613,9 @@ void rows_kernel(const RowsParams p) {
   lds_barrier();
   auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
     constexpr int stage = decltype(stage_tag)::value;
-    const int k0 = plan.tile(t) * BN;
+    const int e0 = t * BN;
     if (t + 1 < t1) src.fetch(t + 1, stage ^ 1);
-    if (k0 <= whi && (k0 + BN > wlo - p.window + 1 || k0 < p.sinks)) {
+    if (plan.key(e0) <= whi && (plan.key(e0 + BN - 1) > wlo - p.window || plan.key(e0) < p.sinks)) {
       const uint16_t *kt = src.keys(stage), *vt = src.values(stage);
       f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -617,12 +623,13 @@ void rows_kernel(const RowsParams p) {
         s[0] = E::mma(lds_row_chunk<D>(kt, perm_row(c), m, g), q[m], s[0]);
         s[1] = E::mma(lds_row_chunk<D>(kt, 32 + perm_row(c), m, g), q[m], s[1]);
       }
-      if (!(k0 + BN - 1 <= wlo && (k0 > whi - p.window || k0 + BN <= p.sinks))) {
+      sched_score_tile<KS, 0>();
+      if (!rows_full(p, plan, wlo, whi, e0, BN)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!row_sees(p, pos, k0 + 32 * kb + acc_row(r, g))) s[kb][r] = neg_inf();
+            if (!row_sees(p, pos, plan.key(e0 + 32 * kb + acc_row(r, g)))) s[kb][r] = neg_inf();
       }
       u32x4 pb[4];
       a.tile(s, p.qk_scale, pb);
@@ -634,7 +641,7 @@ void rows_kernel(const RowsParams p) {
       if constexpr (SRC::kNanBlocks) {
         const uint32_t nan = src.nan_blocks(stage, lane);
         if (__builtin_amdgcn_ballot_w64(nan != 0) != 0)
-          set_nan_rows(a, p, pos, k0, [&](int row) {
+          set_nan_rows(a, p, plan, pos, e0, [&](int row) {
             return (uint32_t)__builtin_amdgcn_readlane((int)nan, row);
           });
       }

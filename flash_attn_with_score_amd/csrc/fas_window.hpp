@@ -15,8 +15,9 @@
 //                         to as many workgroups as make them about equal;
 //                         they write fp32 parts that window_reduce_kernel
 //                         adds in order.
-//   window_dq_kernel      query-block outer: tiles of 64 keys, the sinks' first,
-//                         then the window's: S^T, P^T, dS^T, dQ^T += K^T dS^T.
+//   window_dq_kernel      query-block outer, over tiles of 64 entries of the key
+//                         list that RowsPlan describes: S^T, P^T, dS^T,
+//                         dQ^T += K^T dS^T.
 //
 // A pair that a row does not see has P = 0 and so dS = 0; P and dS are rounded
 // to the input type for their products, everything else is fp32.
@@ -51,12 +52,22 @@ struct DenseSource {
         sv(p.sv2 >> 1), wave(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)),
         lane((int)threadIdx.x & 63) {}
   __device__ __forceinline__ void fetch(int t, int stage) {
-    const int r0 = plan.tile(t) * kRowsKeys;
     // (The descriptors are uniform, but at D = 16, where half the waves load,
     // the compiler moves them to vector registers.)
     const i32x4 wk = uniform(wk_), wv = uniform(wv_);
-    dma_tile<D, kRowsKeys, 4>(wk, sk, r0, lds_addr(lds.kv[stage][0]), wave, lane);
-    dma_tile<D, kRowsKeys, 4>(wv, sv, r0, lds_addr(lds.kv[stage][1]), wave, lane);
+    constexpr int BLOCKS = TILE / 512, RPB = 512 / D, CPR = D / 8;  // as dma_tile
+#pragma unroll
+    for (int i = 0; i < (BLOCKS + 3) / 4; ++i) {
+      const int q = wave + 4 * i;
+      if (BLOCKS % 4 == 0 || q < BLOCKS) {
+        const int row = q * RPB + lane / CPR, ch = (lane % CPR) ^ swz<D>(row);
+        const int key = plan.key(t * kRowsKeys + row);
+        dma16(wk, (uint32_t)(key * sk + ch * 8) * 2u,
+              __builtin_amdgcn_readfirstlane(lds_addr(lds.kv[stage][0]) + (uint32_t)(q * 1024)));
+        dma16(wv, (uint32_t)(key * sv + ch * 8) * 2u,
+              __builtin_amdgcn_readfirstlane(lds_addr(lds.kv[stage][1]) + (uint32_t)(q * 1024)));
+      }
+    }
   }
   __device__ __forceinline__ void land(int) { vm_wait_all(); }
   __device__ __forceinline__ const uint16_t* keys(int stage) const { return lds.kv[stage][0]; }
@@ -84,17 +95,17 @@ struct DenseFewSource {
     return D >= 32 ? 32 * m + 8 * g : 8 * (g & 1);
   }
   __device__ __forceinline__ void fetch(int t) {
-    const int k0 = plan.tile(t) * kFewKeys;
+    const int e0 = t * kFewKeys;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint8_t* row = kp + (int64_t)min(k0 + 16 * i + c, plan.len - 1) * sk;
+      const uint8_t* row = kp + (int64_t)plan.row(e0 + 16 * i + c) * sk;
 #pragma unroll
       for (int m = 0; m < KS; ++m) k[i][m] = *reinterpret_cast<const u32x4*>(row + 64 * m);
     }
 #pragma unroll
     for (int j = 0; j < VL; ++j)
       v[j] = *reinterpret_cast<const u32x4*>(
-          vp + (int64_t)min(k0 + value_row(j), plan.len - 1) * sv);
+          vp + (int64_t)plan.row(e0 + value_row(j)) * sv);
   }
   __device__ __forceinline__ int value_row(int j) const { return (64 * j + lane) / (D / 8); }
   __device__ __forceinline__ void take() {}
@@ -398,24 +409,35 @@ void window_dq_kernel(const WindowBwdParams p) {
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]), "+v"(greg[ks]));
 
-  // Key tiles of the block: the sinks' before the window, then the window's.
+  // The block's keys as a list, as RowsPlan has it: ns sinks, then the window.
   const int lo = p.causal_off + row0, hi = min(p.N - 1, lo + BM - 1);
-  int sink_tiles = 0, win = 0, ntiles = 0;
+  int ns = 0, shift = 0, ntiles = 0;
   if (hi >= 0) {
-    win = max(0, lo - p.window + 1) / BN;
-    sink_tiles = min(win, (min(p.sinks, hi + 1) + BN - 1) / BN);
-    ntiles = sink_tiles + (hi + BN) / BN - win;
+    const int first = max(0, lo - p.window + 1);
+    ns = min(first, p.sinks);
+    shift = first - ns;
+    ntiles = (hi + 1 - shift + BN - 1) / BN;
   }
+  auto key_of = [&](int e) __attribute__((always_inline)) { return e < ns ? e : e + shift; };
   const int wlo = p.causal_off + wrow0, whi = wrow0 < p.M ? min(p.N - 1, wlo + 31) : -1;
   const int pos = p.causal_off + qrow;
 
   const i32x4 wk = make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
   const i32x4 wv = make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
   const uint32_t k_base = lds_addr(&klds[0][0]), v_base = lds_addr(&vlds[0][0]);
-  auto tile_key = [&](int t) { return (t < sink_tiles ? t : t - sink_tiles + win) * BN; };
   auto fetch = [&](int t, int s) __attribute__((always_inline)) {
-    dma_tile<D, BN, NW>(wk, p.sk2, tile_key(t), k_base + (uint32_t)(s * TILE * 2), wave, lane);
-    dma_tile<D, BN, NW>(wv, p.sv2, tile_key(t), v_base + (uint32_t)(s * TILE * 2), wave, lane);
+    constexpr int BLOCKS = TILE / 512, RPB = 512 / D, CPR = D / 8;  // as dma_tile
+#pragma unroll
+    for (int i = 0; i < (BLOCKS + NW - 1) / NW; ++i) {
+      const int q = wave + NW * i;
+      if (BLOCKS % NW == 0 || q < BLOCKS) {
+        const int row = q * RPB + lane / CPR, ch = (lane % CPR) ^ swz<D>(row);
+        const int key = key_of(t * BN + row);
+        const uint32_t lb = (uint32_t)(s * TILE * 2 + q * 1024);
+        dma16(wk, (uint32_t)(key * p.sk2 + ch * 8) * 2u, __builtin_amdgcn_readfirstlane(k_base + lb));
+        dma16(wv, (uint32_t)(key * p.sv2 + ch * 8) * 2u, __builtin_amdgcn_readfirstlane(v_base + lb));
+      }
+    }
   };
 
   f32x16 dq[DB];
@@ -436,10 +458,9 @@ void window_dq_kernel(const WindowBwdParams p) {
     if (more) fetch(t + 1, stage ^ 1);
     const uint16_t* kt = klds[stage];
     const uint16_t* vt = vlds[stage];
-    const int k0 = tile_key(t);
+    const int e0 = t * BN;
     // One 32-key sub-block (bwd_dq_kernel has the reasons for its fences).
     auto body = [&](int kb2, bool full) __attribute__((always_inline)) {
-      const int kbase = k0 + 32 * kb2;
       __builtin_amdgcn_sched_barrier(0);
       uint32_t ro = rco;
       opaque(ro);
@@ -449,7 +470,7 @@ void window_dq_kernel(const WindowBwdParams p) {
         ak[ks] = lds_row_chunk(kt + 32 * kb2 * D, ro, ks);
         av[ks] = lds_row_chunk(vt + 32 * kb2 * D, ro, ks);
       }
-      // Register r holds key kbase + acc_row(r, g) for query row qrow.
+      // Register r holds list entry e0 + 32 kb2 + acc_row(r, g) for query row qrow.
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = xl;
@@ -474,7 +495,7 @@ void window_dq_kernel(const WindowBwdParams p) {
       for (int r = 0; r < 16; ++r) {
         pr[r] = exp2f_fast(fmaf(s[r], qk, nl));
         if (!full) {
-          const int key = kbase + acc_row(r, g);
+          const int key = key_of(e0 + 32 * kb2 + acc_row(r, g));
           if (key > pos || (key <= pos - p.window && key >= p.sinks)) pr[r] = 0.f;
         }
       }
@@ -500,9 +521,12 @@ void window_dq_kernel(const WindowBwdParams p) {
     };
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
-      const int kbase = k0 + 32 * kb2;
-      const bool live = kbase <= whi && (kbase + 32 > wlo - p.window + 1 || kbase < p.sinks);
-      const bool full = kbase + 31 <= wlo && (kbase > whi - p.window || kbase + 32 <= p.sinks);
+      // The sub-block's first and last keys (a tile that the sinks end in holds
+      // keys of both kinds).
+      const int e = e0 + 32 * kb2, ka = key_of(e), kz = key_of(e + 31);
+      const bool live = ka <= whi && (kz > wlo - p.window || ka < p.sinks);
+      const bool full = kz <= wlo && (e + 32 <= ns || max(e, ns) + shift > whi - p.window ||
+                                      kz < p.sinks);
       if (live) body(kb2, full);
     }
     if (more) vm_wait_all();
