@@ -337,7 +337,7 @@ __device__ __forceinline__ int acc_row(int r, int g) { return 16 * (r >> 3) + 8 
 // from 16 consecutive rows (ds_read_b128), and 32 lanes reading 4 rows x 64
 // bytes with the transposing ds_read_b64_tr_b16.
 template <int D>
-__device__ __forceinline__ int swz(int row) {
+__host__ __device__ __forceinline__ constexpr int swz(int row) {
   if constexpr (D == 128) {
     return ((row & 3) << 2) | ((row >> 2) & 3);
   } else if constexpr (D == 64) {

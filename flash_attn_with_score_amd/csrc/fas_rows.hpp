@@ -45,6 +45,7 @@ struct RowsPlan {
   int len, cnt, pos0;  // keys, query rows, position of row 0
   int lo, hi;          // least and greatest position of the block's live rows (hi < lo: none)
   int ns, shift;       // entry e is key e, or e + shift from entry ns on
+  int hide;            // entries in front of this one are sinks: the window's edge leaves them
   int tiles, per, used;
   __device__ __forceinline__ int key(int e) const { return e < ns ? e : e + shift; }
   // The key whose row stands in for entry e in memory: entries behind the
@@ -61,11 +62,12 @@ __device__ __forceinline__ RowsPlan rows_tiles(const RowsParams& p, int b, int r
   const int i0 = rb * BM / p.G, i1 = min(c.cnt, (rb * BM + BM - 1) / p.G + 1);  // rows [i0, i1)
   c.lo = c.pos0 + i0;
   c.hi = i1 > i0 ? c.pos0 + i1 - 1 : c.lo - 1;
-  c.ns = c.shift = c.tiles = 0;
+  c.ns = c.shift = c.hide = c.tiles = 0;
   if (c.hi >= max(c.lo, 0)) {
     const int first = max(0, max(c.lo, 0) - p.window + 1);
     c.ns = min(first, p.sinks);
     c.shift = first - c.ns;
+    c.hide = c.shift > 0 ? c.ns : p.sinks;
     c.tiles = (c.hi + 1 - c.shift + BN - 1) / BN;
   }
   return c;
@@ -129,7 +131,7 @@ __device__ __forceinline__ RowsPlan rows_balanced(const RowsParams& p, int id, i
   if (b < p.B) {
     auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
     c = RowsPlan{of(c.len), of(c.cnt), of(c.pos0), of(c.lo), of(c.hi), of(c.ns), of(c.shift),
-                 of(c.tiles), per, of(used)};
+                 of(c.hide), of(c.tiles), per, of(used)};
     const int rest = id - (of(end) - c.used * p.Hk);
     hk = __builtin_amdgcn_readfirstlane(rest / c.used);
     split = rest - hk * c.used;
@@ -138,14 +140,33 @@ __device__ __forceinline__ RowsPlan rows_balanced(const RowsParams& p, int id, i
   return c;
 }
 
-// Whether rows at positions [lo, hi] all see entries [e0, e0 + n).
-__device__ __forceinline__ bool rows_full(const RowsParams& p, const RowsPlan& c, int lo, int hi,
-                                          int e0, int n) {
-  return c.key(e0 + n - 1) <= lo &&
-         (e0 + n <= c.ns || max(e0, c.ns) + c.shift > hi - p.window || c.key(e0 + n - 1) < p.sinks);
+// Which entries of the list the row at position pos sees: all up to
+// pos - shift but those in [hide, pos - window - shift].  (Sinks stand in front
+// of every row's own position: ns <= lo - shift.)
+struct RowMask {
+  int last;   // last visible entry
+  int first;  // first entry behind `hide` that is not in front of the window
+  __device__ __forceinline__ RowMask(const RowsParams& p, const RowsPlan& c, int pos)
+      : last(pos - c.shift), first(pos - p.window - c.shift + 1) {}
+};
+// What a tile of entries [e0, e0 + n) needs for rows at positions [lo, hi]:
+// whether some row does not see its end, or its entries in front of a window.
+struct TileMask {
+  bool end, edge;
+  __device__ __forceinline__ TileMask(const RowsParams& p, const RowsPlan& c, int lo, int hi, int e0,
+                                      int n)
+      : end(e0 + n - 1 > lo - c.shift),
+        edge(e0 + n > c.hide && max(e0, c.hide) < hi - p.window - c.shift + 1) {}
+};
+// Score s of entry e under the masks that its tile needs.
+__device__ __forceinline__ float masked_score(float s, int e, const RowMask& m, const RowsPlan& c,
+                                              bool end, bool edge) {
+  if (end) s = e > m.last ? neg_inf() : s;
+  if (edge) s = (uint32_t)(e - c.hide) < (uint32_t)max(0, m.first - c.hide) ? neg_inf() : s;
+  return s;
 }
-__device__ __forceinline__ bool row_sees(const RowsParams& p, int pos, int key) {
-  return key <= pos && (key > pos - p.window || key < p.sinks);
+__device__ __forceinline__ bool row_sees(const RowMask& m, const RowsPlan& c, int e) {
+  return e <= m.last && (e < c.hide || e >= m.first);
 }
 
 // Online softmax of one row a lane pair (lanes c and c + 32) over tiles of
@@ -208,11 +229,11 @@ struct SoftRows {
 // NaN blocks: bit `group` of flag(row) says that the V block of tile row `row`
 // reads as NaN; rows that see the key are set to NaN there.
 template <class E, int D, int NB, class F>
-__device__ __forceinline__ void set_nan_rows(SoftRows<E, D, NB>& a, const RowsParams& p,
-                                              const RowsPlan& plan, int pos, int e0, F&& flag) {
+__device__ __forceinline__ void set_nan_rows(SoftRows<E, D, NB>& a, const RowMask& m,
+                                             const RowsPlan& plan, int e0, F&& flag) {
   for (int row = 0; row < 32 * NB; ++row) {
     const uint32_t f = flag(row);
-    const bool sees = row_sees(p, pos, plan.key(e0 + row));
+    const bool sees = row_sees(m, plan, e0 + row);
 #pragma unroll
     for (int db = 0; db < SoftRows<E, D, NB>::DB; ++db)
       if ((f >> db) & 1u)
@@ -281,6 +302,39 @@ __device__ __forceinline__ u32x4 load_q(const RowsParams& p, int b, int hk, int 
   return *reinterpret_cast<const u32x4*>(p.q + b * p.sq0 + h * p.sq1 + (int64_t)i * p.sq2 + d0) ^
          p.qneg;
 }
+
+// LDS DMA of tiles of 64 rows of D 16-bit elements by four waves, as dma_tile,
+// with the addresses reduced to one add a transfer: the rows that a lane
+// fetches lie 2048 / D apart, which the swizzle does not see, so its offset is
+// one per-lane part and uniform ones.
+template <int D>
+struct TileDma {
+  static constexpr int BLOCKS = 64 * D / 512, RPB = 512 / D, CPR = D / 8;
+  static_assert(BLOCKS <= 4 || swz<D>(0) == swz<D>(4 * RPB), "the swizzle's period");
+  int wave, row;   // the lane's first row
+  uint32_t lane;   // byte offset of its 16 bytes in a tile
+  uint32_t step;   // bytes from one of its rows to the next
+  uint32_t pitch;  // bytes of a row
+  __device__ __forceinline__ TileDma(int wave_, int l, uint32_t stride)
+      : wave(wave_), row(wave_ * RPB + l / CPR), pitch(2u * stride) {
+    lane = (uint32_t)row * pitch + (uint32_t)(((l % CPR) ^ swz<D>(row)) << 4);
+    step = 4u * RPB * pitch;
+  }
+  // Entries [e0, e0 + 64) of the list: rows e0 .., or `shift` rows on from
+  // entry ns.
+  __device__ __forceinline__ void fetch(i32x4 rsrc, int e0, int ns, int shift, uint32_t lds) const {
+    const bool mixed = e0 < ns && e0 + 64 > ns;
+    const uint32_t base = (uint32_t)(e0 + (e0 >= ns ? shift : 0)) * pitch;
+#pragma unroll
+    for (int i = 0; i < (BLOCKS + 3) / 4; ++i) {
+      if (BLOCKS % 4 == 0 || wave + 4 * i < BLOCKS) {
+        uint32_t off = lane + (base + (uint32_t)i * step);
+        if (mixed && e0 + row + 4 * RPB * i >= ns) off += (uint32_t)shift * pitch;
+        dma16(rsrc, off, __builtin_amdgcn_readfirstlane(lds + (uint32_t)((wave + 4 * i) * 1024)));
+      }
+    }
+  }
+};
 
 // ---------------------------------------------------------------- few rows
 
@@ -474,13 +528,15 @@ void few_kernel(const RowsParams p) {
 #pragma unroll
         for (int n = 0; n < NC; ++n) s[n][i] = mma16(E{}, k, q[n][m], s[n][i]);
       }
-    if (!rows_full(p, plan, plan.lo, plan.hi, e0, BN)) {
+    const TileMask need(p, plan, plan.lo, plan.hi, e0, BN);
+    if (need.end || need.edge) {
 #pragma unroll
       for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (!row_sees(p, pos[n], plan.key(e0 + 16 * (e >> 2) + 4 * g + (e & 3))))
-            s[n][e >> 2][e & 3] = neg_inf();
+          s[n][e >> 2][e & 3] =
+              masked_score(s[n][e >> 2][e & 3], e0 + 16 * (e >> 2) + 4 * g + (e & 3),
+                           RowMask(p, plan, pos[n]), plan, true, true);
     }
     // A wave's LDS accesses run in issue order: only the compiler must keep the
     // last tile's reads, these writes and the reads below in theirs.
@@ -511,7 +567,7 @@ void few_kernel(const RowsParams p) {
           if (f == 0) continue;
 #pragma unroll
           for (int n = 0; n < NC; ++n) {
-            const bool sees = row_sees(p, pos[n], plan.key(e0 + row));
+            const bool sees = row_sees(RowMask(p, plan, pos[n]), plan, e0 + row);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
               if ((f >> (dt / 2)) & 1u)
@@ -604,6 +660,16 @@ void rows_kernel(const RowsParams p) {
 #pragma unroll
   for (int m = 0; m < KS; ++m) q[m] = load_q<D>(p, b, hk, v, 16 * m + 8 * g);
 
+  const RowMask mask(p, plan, pos);
+  // In tiles of the list: the wave's rows see nothing from tile w_end on nor in
+  // tiles [w_hide, w_first); tiles before w_edge may cross a row's window, those
+  // from w_last on a row's own position; the others need no mask.
+  const int first = wlo - p.window - plan.shift + 1;
+  const int w_end = whi < 0 ? 0 : (whi - plan.shift) / BN + 1;
+  const int w_hide = (plan.hide + BN - 1) / BN, w_first = max(0, first) / BN;
+  const int w_edge = (max(0, whi - p.window - plan.shift + 1) + BN - 1) / BN;
+  const int w_last = max(0, wlo - plan.shift + 1) / BN;
+
   SRC src(p, plan, b, hk, lds);
   SoftRows<E, D, 2> a;
   if (t0 < t1) {
@@ -615,7 +681,7 @@ void rows_kernel(const RowsParams p) {
     constexpr int stage = decltype(stage_tag)::value;
     const int e0 = t * BN;
     if (t + 1 < t1) src.fetch(t + 1, stage ^ 1);
-    if (plan.key(e0) <= whi && (plan.key(e0 + BN - 1) > wlo - p.window || plan.key(e0) < p.sinks)) {
+    if (t < w_end && !(t >= w_hide && t < w_first)) {
       const uint16_t *kt = src.keys(stage), *vt = src.values(stage);
       f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -624,13 +690,17 @@ void rows_kernel(const RowsParams p) {
         s[1] = E::mma(lds_row_chunk<D>(kt, 32 + perm_row(c), m, g), q[m], s[1]);
       }
       sched_score_tile<KS, 0>();
-      if (!rows_full(p, plan, wlo, whi, e0, BN)) {
+      // (A copy of the step without these branches needs more registers than
+      // two waves a SIMD have.)
+      auto apply = [&](bool end, bool edge) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!row_sees(p, pos, plan.key(e0 + 32 * kb + acc_row(r, g)))) s[kb][r] = neg_inf();
-      }
+            s[kb][r] = masked_score(s[kb][r], e0 + 32 * kb + acc_row(r, g), mask, plan, end, edge);
+      };
+      if (t >= w_last) apply(true, false);
+      if (t < w_edge) apply(false, true);
       u32x4 pb[4];
       a.tile(s, p.qk_scale, pb);
 #pragma unroll
@@ -641,7 +711,7 @@ void rows_kernel(const RowsParams p) {
       if constexpr (SRC::kNanBlocks) {
         const uint32_t nan = src.nan_blocks(stage, lane);
         if (__builtin_amdgcn_ballot_w64(nan != 0) != 0)
-          set_nan_rows(a, p, plan, pos, e0, [&](int row) {
+          set_nan_rows(a, mask, plan, e0, [&](int row) {
             return (uint32_t)__builtin_amdgcn_readlane((int)nan, row);
           });
       }

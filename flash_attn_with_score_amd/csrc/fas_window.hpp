@@ -37,9 +37,8 @@ struct DenseSource {
   };
   Lds& lds;
   const RowsPlan& plan;
-  const i32x4 wk_, wv_;
-  const int64_t sk, sv;
-  const int wave, lane;
+  const i32x4 wk, wv;
+  const TileDma<D> dk, dv;
   static __device__ __forceinline__ i32x4 uniform(i32x4 w) {
     return i32x4{__builtin_amdgcn_readfirstlane(w.x), __builtin_amdgcn_readfirstlane(w.y),
                  __builtin_amdgcn_readfirstlane(w.z), __builtin_amdgcn_readfirstlane(w.w)};
@@ -47,27 +46,16 @@ struct DenseSource {
   __device__ __forceinline__ DenseSource(const RowsParams& p, const RowsPlan& plan_, int b, int hk,
                                          Lds& lds_)
       : lds(lds_), plan(plan_),
-        wk_(make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes)),
-        wv_(make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes)), sk(p.sk2 >> 1),
-        sv(p.sv2 >> 1), wave(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)),
-        lane((int)threadIdx.x & 63) {}
+        wk(make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes)),
+        wv(make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes)),
+        dk(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), (int)threadIdx.x & 63,
+           (uint32_t)(p.sk2 >> 1)),
+        dv(dk.wave, (int)threadIdx.x & 63, (uint32_t)(p.sv2 >> 1)) {}
   __device__ __forceinline__ void fetch(int t, int stage) {
     // (The descriptors are uniform, but at D = 16, where half the waves load,
     // the compiler moves them to vector registers.)
-    const i32x4 wk = uniform(wk_), wv = uniform(wv_);
-    constexpr int BLOCKS = TILE / 512, RPB = 512 / D, CPR = D / 8;  // as dma_tile
-#pragma unroll
-    for (int i = 0; i < (BLOCKS + 3) / 4; ++i) {
-      const int q = wave + 4 * i;
-      if (BLOCKS % 4 == 0 || q < BLOCKS) {
-        const int row = q * RPB + lane / CPR, ch = (lane % CPR) ^ swz<D>(row);
-        const int key = plan.key(t * kRowsKeys + row);
-        dma16(wk, (uint32_t)(key * sk + ch * 8) * 2u,
-              __builtin_amdgcn_readfirstlane(lds_addr(lds.kv[stage][0]) + (uint32_t)(q * 1024)));
-        dma16(wv, (uint32_t)(key * sv + ch * 8) * 2u,
-              __builtin_amdgcn_readfirstlane(lds_addr(lds.kv[stage][1]) + (uint32_t)(q * 1024)));
-      }
-    }
+    dk.fetch(uniform(wk), t * kRowsKeys, plan.ns, plan.shift, lds_addr(lds.kv[stage][0]));
+    dv.fetch(uniform(wv), t * kRowsKeys, plan.ns, plan.shift, lds_addr(lds.kv[stage][1]));
   }
   __device__ __forceinline__ void land(int) { vm_wait_all(); }
   __device__ __forceinline__ const uint16_t* keys(int stage) const { return lds.kv[stage][0]; }
@@ -194,6 +182,7 @@ void window_dkdv_kernel(const WindowBwdParams p) {
   // < reach (a key past N: never).
   const int reach = key0 + c >= p.N ? 0 : key0 + c < p.sinks ? 0x7fffffff : p.window;
 
+  const TileDma<D> qdma(wave, lane, (uint32_t)p.sq2), gdma(wave, lane, (uint32_t)p.sg2);
   for (int hh = 0; hh < p.G; ++hh) {
     const int t0 = tlo + max(0, s0 - hh * tiles), t1 = tlo + min(tiles, s1 - hh * tiles);
     if (t0 >= t1) continue;
@@ -205,8 +194,8 @@ void window_dkdv_kernel(const WindowBwdParams p) {
     const float* xg = p.delta + bh * p.Mpad;
     float nst = 0.f, xst = 0.f;
     auto fetch = [&](int t, int s) __attribute__((always_inline)) {
-      dma_tile<D, TQ, NW>(wq, p.sq2, t * TQ, q_base + (uint32_t)(s * TILE * 2), wave, lane);
-      dma_tile<D, TQ, NW>(wg, p.sg2, t * TQ, g_base + (uint32_t)(s * TILE * 2), wave, lane);
+      qdma.fetch(wq, t * TQ, 0, 0, q_base + (uint32_t)(s * TILE * 2));
+      gdma.fetch(wg, t * TQ, 0, 0, g_base + (uint32_t)(s * TILE * 2));
       if (tid < TQ) {
         nst = nlg[t * TQ + tid];
         xst = xg[t * TQ + tid];
@@ -411,11 +400,12 @@ void window_dq_kernel(const WindowBwdParams p) {
 
   // The block's keys as a list, as RowsPlan has it: ns sinks, then the window.
   const int lo = p.causal_off + row0, hi = min(p.N - 1, lo + BM - 1);
-  int ns = 0, shift = 0, ntiles = 0;
+  int ns = 0, shift = 0, hide = 0, ntiles = 0;
   if (hi >= 0) {
     const int first = max(0, lo - p.window + 1);
     ns = min(first, p.sinks);
     shift = first - ns;
+    hide = shift > 0 ? ns : p.sinks;
     ntiles = (hi + 1 - shift + BN - 1) / BN;
   }
   auto key_of = [&](int e) __attribute__((always_inline)) { return e < ns ? e : e + shift; };
@@ -425,19 +415,10 @@ void window_dq_kernel(const WindowBwdParams p) {
   const i32x4 wk = make_rsrc_words(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
   const i32x4 wv = make_rsrc_words(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
   const uint32_t k_base = lds_addr(&klds[0][0]), v_base = lds_addr(&vlds[0][0]);
+  const TileDma<D> dk(wave, lane, (uint32_t)p.sk2), dv(wave, lane, (uint32_t)p.sv2);
   auto fetch = [&](int t, int s) __attribute__((always_inline)) {
-    constexpr int BLOCKS = TILE / 512, RPB = 512 / D, CPR = D / 8;  // as dma_tile
-#pragma unroll
-    for (int i = 0; i < (BLOCKS + NW - 1) / NW; ++i) {
-      const int q = wave + NW * i;
-      if (BLOCKS % NW == 0 || q < BLOCKS) {
-        const int row = q * RPB + lane / CPR, ch = (lane % CPR) ^ swz<D>(row);
-        const int key = key_of(t * BN + row);
-        const uint32_t lb = (uint32_t)(s * TILE * 2 + q * 1024);
-        dma16(wk, (uint32_t)(key * p.sk2 + ch * 8) * 2u, __builtin_amdgcn_readfirstlane(k_base + lb));
-        dma16(wv, (uint32_t)(key * p.sv2 + ch * 8) * 2u, __builtin_amdgcn_readfirstlane(v_base + lb));
-      }
-    }
+    dk.fetch(wk, t * BN, ns, shift, k_base + (uint32_t)(s * TILE * 2));
+    dv.fetch(wv, t * BN, ns, shift, v_base + (uint32_t)(s * TILE * 2));
   };
 
   f32x16 dq[DB];
@@ -460,7 +441,7 @@ void window_dq_kernel(const WindowBwdParams p) {
     const uint16_t* vt = vlds[stage];
     const int e0 = t * BN;
     // One 32-key sub-block (bwd_dq_kernel has the reasons for its fences).
-    auto body = [&](int kb2, bool full) __attribute__((always_inline)) {
+    auto body = [&](int kb2, bool end, bool edge) __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
       uint32_t ro = rco;
       opaque(ro);
@@ -490,14 +471,17 @@ void window_dq_kernel(const WindowBwdParams p) {
           if (i + PD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
       }
+      // RowMask in entries of the sub-block: those past `last`, and those in
+      // [hide, hide + span).
+      const int ebase = e0 + 32 * kb2;
+      const int last = pos - shift - ebase, below = ebase - hide;
+      const int span = max(0, pos - p.window - shift + 1 - hide);
       float pr[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         pr[r] = exp2f_fast(fmaf(s[r], qk, nl));
-        if (!full) {
-          const int key = key_of(e0 + 32 * kb2 + acc_row(r, g));
-          if (key > pos || (key <= pos - p.window && key >= p.sinks)) pr[r] = 0.f;
-        }
+        if (end && acc_row(r, g) > last) pr[r] = 0.f;
+        if (edge && (uint32_t)(acc_row(r, g) + below) < (uint32_t)span) pr[r] = 0.f;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = pr[r] * dp[r];
@@ -521,13 +505,13 @@ void window_dq_kernel(const WindowBwdParams p) {
     };
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
-      // The sub-block's first and last keys (a tile that the sinks end in holds
-      // keys of both kinds).
+      // The sub-block's first and last keys (one that the sinks end in holds
+      // keys of both kinds), and the masks that it needs (TileMask).
       const int e = e0 + 32 * kb2, ka = key_of(e), kz = key_of(e + 31);
-      const bool live = ka <= whi && (kz > wlo - p.window || ka < p.sinks);
-      const bool full = kz <= wlo && (e + 32 <= ns || max(e, ns) + shift > whi - p.window ||
-                                      kz < p.sinks);
-      if (live) body(kb2, full);
+      if (ka > whi || (kz <= wlo - p.window && ka >= p.sinks)) continue;
+      const bool end = e + 31 > wlo - shift;
+      const bool edge = e + 32 > hide && max(e, hide) < whi - p.window - shift + 1;
+      body(kb2, end, edge);
     }
     if (more) vm_wait_all();
     __syncthreads();
