@@ -366,13 +366,13 @@ constexpr int kBalanceBatch = 64;
 constexpr int kNoWindow = 1 << 30;
 
 // Backward of the windowed attention (fas_window.hpp).  part: fp32 dK | dV of
-// the key blocks dealt to several workgroups, slabs of 128 keys x 2D: first
-// the `sink_blocks` blocks that hold sinks (seen by every later row), in
-// sink_pieces each, then the others in `pieces` each where that is more than
-// one.
+// parts of key blocks, slabs of 128 keys x 2D, two for each workgroup of the
+// dK/dV kernel.
 struct WindowBwdParams : BwdParams {
   int window, sinks;
-  int sink_blocks, sink_pieces;
+  int wgs;             // workgroups of the dK/dV kernel
+  int chunk;           // row tiles of each, or 0: a whole key block each
+  int64_t head_tiles;  // row tiles of a KV head's key blocks
 };
 
 }  // namespace fas

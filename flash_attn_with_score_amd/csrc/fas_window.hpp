@@ -10,11 +10,14 @@
 //                         dK^T += Q^T dS.  The rows that see a block of 128
 //                         keys are one run: those at most `window` behind its
 //                         last key, or, where the block holds sinks, all later
-//                         ones.  A block with sinks would take M / (window +
-//                         128) times as long as another, so its run is dealt
-//                         to as many workgroups as make them about equal;
-//                         they write fp32 parts that window_reduce_kernel
-//                         adds in order.
+//                         ones, which is M / (window + 128) times as long.
+//                         So the row tiles of all blocks (of all heads) are one
+//                         list, block after block, and every workgroup takes
+//                         an equal run of it (p.chunk tiles): parts of a block
+//                         at its ends, whole blocks between.  Parts go to fp32
+//                         slabs, two a workgroup, that window_reduce_kernel
+//                         adds in order.  Where whole blocks are even enough
+//                         (p.chunk 0) a workgroup takes one.
 //   window_dq_kernel      query-block outer, over tiles of 64 entries of the key
 //                         list that RowsPlan describes: S^T, P^T, dS^T,
 //                         dQ^T += K^T dS^T.
@@ -105,11 +108,43 @@ struct DenseFewSource {
   }
 };
 
-// Part of the fp32 workspace that piece `piece` of key block kb writes.
-__device__ __forceinline__ int64_t window_slab(const WindowBwdParams& p, int bhk, int kb, int piece) {
-  if (kb < p.sink_blocks) return ((int64_t)bhk * p.sink_blocks + kb) * p.sink_pieces + piece;
-  const int64_t base = p.sink_pieces > 1 ? (int64_t)p.B * p.Hk * p.sink_blocks * p.sink_pieces : 0;
-  return base + ((int64_t)bhk * (p.nkb - p.sink_blocks) + kb - p.sink_blocks) * p.pieces + piece;
+// 64-row tiles (of one query head) that see key block kb: [lo, lo + n).
+__device__ __forceinline__ void window_tiles(const WindowBwdParams& p, int kb, int& lo, int& n) {
+  const int k0 = kb * kBwdBlock, rlo = max(0, k0 - p.causal_off);
+  const int rhi = k0 < p.sinks ? p.M
+                               : (int)min((int64_t)p.M, (int64_t)k0 + kBwdBlock - 1 + p.window -
+                                                            p.causal_off);
+  lo = rlo / 64;
+  n = max(0, (rhi + 63) / 64 - lo);
+}
+// Tiles (of G heads) of key blocks [0, kb) of a KV head, worked out 64 blocks at
+// a time; `find` instead: the block that tile `at` falls into, and the tiles
+// before it.
+__device__ __forceinline__ int64_t window_before(const WindowBwdParams& p, int kb) {
+  const int lane = (int)threadIdx.x & 63;
+  int64_t sum = 0;
+  for (int k = 0; k < kb; k += 64) {
+    int lo, n = 0;
+    if (k + lane < kb) window_tiles(p, k + lane, lo, n);
+    sum += __builtin_amdgcn_readlane(wave_scan(n * p.G, [](int x, int y) { return x + y; }), 63);
+  }
+  return sum;
+}
+__device__ __forceinline__ int window_find(const WindowBwdParams& p, int64_t at, int64_t& before) {
+  const int lane = (int)threadIdx.x & 63;
+  before = 0;
+  for (int k = 0;; k += 64) {
+    int lo, n = 0;
+    if (k + lane < p.nkb) window_tiles(p, k + lane, lo, n);
+    const int end = wave_scan(n * p.G, [](int x, int y) { return x + y; });
+    const int total = __builtin_amdgcn_readlane(end, 63);
+    if (at < before + total || k + 64 >= p.nkb) {
+      const int i = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + end <= at));
+      if (i > 0) before += __builtin_amdgcn_readlane(end, min(i, 64) - 1);
+      return min(k + i, p.nkb - 1);
+    }
+    before += total;
+  }
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -132,19 +167,39 @@ void window_dkdv_kernel(const WindowBwdParams p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, c = lane & 31, g = lane >> 5;
-  // The sinks' pieces first, then the other blocks'.
-  const int nbh = p.B * p.Hk;
-  int id = blockIdx.x, kb, pieces = p.sink_pieces;
-  const int nsink = p.sink_blocks * pieces * nbh;
-  if (id >= nsink) {
-    id -= nsink;
-    pieces = p.pieces;
-    kb = p.sink_blocks + id / (nbh * pieces);
+  // Runs of the list that follow each other go to one XCD (workgroup i runs on
+  // XCD i % 8): they share query rows in its L2.
+  int wg = blockIdx.x;
+  if (gridDim.x % 8 == 0) wg = (wg & 7) * ((int)gridDim.x >> 3) + (wg >> 3);
+  int64_t at = 0, stop = 0, before = 0;  // tiles of the list; those before block kb of this KV head
+  int bhk, kb;
+  if (p.chunk > 0) {
+    at = (int64_t)wg * p.chunk;
+    stop = min(at + p.chunk, (int64_t)p.B * p.Hk * p.head_tiles);
+    if (at >= stop) return;
+    bhk = (int)(at / p.head_tiles);
+    kb = window_find(p, at - (int64_t)bhk * p.head_tiles, before);
   } else {
-    kb = id / (nbh * pieces);
+    wg = blockIdx.x;  // longest first: blocks with sinks
+    kb = wg / (p.B * p.Hk);
+    bhk = wg - kb * (p.B * p.Hk);
   }
-  const int rest = id % (nbh * pieces);
-  const int piece = rest % pieces, bhk = rest / pieces;
+  const float qk = p.qk_scale;
+  const uint32_t q_base = lds_addr(&qlds[0][0]), g_base = lds_addr(&glds[0][0]);
+  const TileDma<D> qdma(wave, lane, (uint32_t)p.sq2), gdma(wave, lane, (uint32_t)p.sg2);
+
+  for (;;) {  // one key block, or the part of it in this workgroup's run
+  bhk = __builtin_amdgcn_readfirstlane(bhk);
+  kb = __builtin_amdgcn_readfirstlane(kb);
+  int tlo, tiles;
+  window_tiles(p, kb, tlo, tiles);
+  // Tiles [s0, s1) of the block's G * tiles, in head order.
+  int s0 = 0, s1 = p.G * tiles;
+  const int64_t start = (int64_t)bhk * p.head_tiles + before;  // the block's first in the list
+  if (p.chunk > 0) {
+    s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
+    s1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)s1, stop - start));
+  }
   const int b = bhk / p.Hk, hk = bhk % p.Hk;
   const int h0 = hk * p.G;
   const int key0 = kb * BK + 32 * wave;  // this wave's keys [key0, key0 + 32)
@@ -167,22 +222,12 @@ void window_dkdv_kernel(const WindowBwdParams p) {
     dv[db] = f32x16{};
   }
 
-  // Query rows [rlo, rhi) that see a key of the block.
-  const int rlo = max(0, kb * BK - p.causal_off);
-  const int rhi = kb * BK < p.sinks ? p.M
-                                    : min((int64_t)p.M, (int64_t)kb * BK + BK - 1 + p.window - p.causal_off);
-  const int tlo = rlo / TQ, tiles = max(0, (rhi + TQ - 1) / TQ - tlo);
-  // This piece's tiles [s0, s1) of the G heads' tiles in head order.
-  int s0, s1;
-  deal(p.G * tiles, piece, pieces, s0, s1);
-  s1 += s0;
-  const float qk = p.qk_scale;
-  const uint32_t q_base = lds_addr(&qlds[0][0]), g_base = lds_addr(&glds[0][0]);
   // Row position - key, per lane: a row sees key key0 + c iff 0 <= difference
   // < reach (a key past N: never).
+  const VtOff vto = vt_offsets<D>(lane);
+  const uint32_t rco = row_chunk_offset<D>(perm_row(c), g);
   const int reach = key0 + c >= p.N ? 0 : key0 + c < p.sinks ? 0x7fffffff : p.window;
 
-  const TileDma<D> qdma(wave, lane, (uint32_t)p.sq2), gdma(wave, lane, (uint32_t)p.sg2);
   for (int hh = 0; hh < p.G; ++hh) {
     const int t0 = tlo + max(0, s0 - hh * tiles), t1 = tlo + min(tiles, s1 - hh * tiles);
     if (t0 >= t1) continue;
@@ -221,51 +266,94 @@ void window_dkdv_kernel(const WindowBwdParams p) {
       // join before the dV / dK products.
       auto body = [&](int qb, bool full) __attribute__((always_inline)) {
         const int r0 = t * TQ + 32 * qb;
-        // Register r holds query row r0 + acc_row(r, g) and key key0 + c.
-        f32x16 s = f32x16{}, dp;
+        // Register r holds query row r0 + acc_row(r, g) and key key0 + c.  One
+        // wave a SIMD runs at D = 128, so nothing covers the wait for an
+        // operand: fetches go two k-steps ahead of the products that take
+        // them, and S and dP alternate.
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t ro = rco;
+        opaque(ro);
+        f32x16 s = f32x16{}, dp, nl;
         load8(dp, &xlds[stage][32 * qb + 8 * g], 0, 0);
         load8(dp, &xlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+        u32x4 aq[KS], ag[KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          s = E::mma(lds_row_chunk<D>(qt, 32 * qb + perm_row(c), ks, g), kreg[ks], s);
+        for (int ks = 0; ks < KS; ++ks) {
+          aq[ks] = lds_row_chunk(qt + 32 * qb * D, ro, ks);
+          ag[ks] = lds_row_chunk(gt + 32 * qb * D, ro, ks);
+        }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          dp = E::mma(lds_row_chunk<D>(gt, 32 * qb + perm_row(c), ks, g), vreg[ks], dp);
-        f32x16 nl;
+        for (int ks = 0; ks < KS; ++ks) {
+          s = E::mma(aq[ks], kreg[ks], s);
+          dp = E::mma(ag[ks], vreg[ks], dp);
+        }
         load8(nl, &nlds[stage][32 * qb + 8 * g], 0, 0);
         load8(nl, &nlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+        {
+          constexpr int PD = KS < 3 ? KS : 3;
+          __builtin_amdgcn_sched_group_barrier(0x100, 4 + 2 * PD, 0);  // DS read
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
+            if (i + PD < KS)
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            else if (i + PD == KS)
+              __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        VtOff vo = vto;
+        opaque(vo);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2f_fast(fmaf(s[r], qk, nl[r]));
         if (!full) {
-          const int diff = p.causal_off + r0 - (key0 + c);
+          int diff = p.causal_off + r0 - (key0 + c);
+          asm volatile("" : "+v"(diff));  // (a branch, not 32 selects on every block)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if ((uint32_t)(diff + acc_row(r, g)) >= (uint32_t)reach) s[r] = 0.f;
         }
+        u32x4 tg[2 * DB], tq[2 * DB];
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tg[2 * db + h] = lds_vt_operand<D>(gt, vo, db, 2 * qb + h);
+            tq[2 * db + h] = lds_vt_operand<D>(qt, vo, db, 2 * qb + h);
+          }
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-        const u32x4 pb0 = pack_b<E>(s, 0), pb1 = pack_b<E>(s, 1);
-        const u32x4 sb0 = pack_b<E>(dp, 0), sb1 = pack_b<E>(dp, 1);
+        const u32x4 pb[2] = {pack_b<E>(s, 0), pack_b<E>(s, 1)};
+        const u32x4 sb[2] = {pack_b<E>(dp, 0), pack_b<E>(dp, 1)};
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          dv[db] = E::mma(lds_vt_operand<D>(gt, db, 2 * qb, lane), pb0, dv[db]);
-          dv[db] = E::mma(lds_vt_operand<D>(gt, db, 2 * qb + 1, lane), pb1, dv[db]);
-        }
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          dk[db] = E::mma(lds_vt_operand<D>(qt, db, 2 * qb, lane), sb0, dk[db]);
-          dk[db] = E::mma(lds_vt_operand<D>(qt, db, 2 * qb + 1, lane), sb1, dk[db]);
+          for (int h = 0; h < 2; ++h) {
+            dv[db] = E::mma(tg[2 * db + h], pb[h], dv[db]);
+            dk[db] = E::mma(tq[2 * db + h], sb[h], dk[db]);
+          }
+        {
+          constexpr int PD = 2;  // operand pairs ahead
+          __builtin_amdgcn_sched_group_barrier(0x100, 4 * PD, 0);
+#pragma unroll
+          for (int i = 0; i < 2 * DB; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            if (i + PD < 2 * DB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+          }
         }
       };
+      // Positions p0 .. p0 + 31 against the wave's keys.
+      auto live = [&](int p0) {
+        return p0 + 31 >= key0 && (key0 + 31 > p0 - p.window || key0 < p.sinks);
+      };
+      auto full = [&](int p0) {
+        return p0 >= key0 + 31 && key0 + 31 < p.N &&
+               (key0 > p0 + 31 - p.window || key0 + 32 <= p.sinks);
+      };
+      const int p0 = p.causal_off + t * TQ;
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        // Positions p0 .. p0 + 31 against the wave's keys.
-        const int p0 = p.causal_off + t * TQ + 32 * qb;
-        const bool live = p0 + 31 >= key0 && (key0 + 31 > p0 - p.window || key0 < p.sinks);
-        const bool full = p0 >= key0 + 31 && key0 + 31 < p.N &&
-                          (key0 > p0 + 31 - p.window || key0 + 32 <= p.sinks);
-        if (live) body(qb, full);
-      }
+      for (int qb = 0; qb < 2; ++qb)
+        if (live(p0 + 32 * qb)) body(qb, full(p0 + 32 * qb));
       if (more) {
         vm_wait_all();
         stash(stage ^ 1);
@@ -281,24 +369,27 @@ void window_dkdv_kernel(const WindowBwdParams p) {
   // Lane (c, g), register r of block db: key key0 + c, head dim
   // 32db + acc_row(r, g).
   const int key = key0 + c;
-  if (key >= p.N) return;
   const float ks_ = p.scale_signed;
-  if (pieces == 1) {
-    uint16_t* dkr = p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2;
-    uint16_t* dvr = p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2;
+  if (s0 == 0 && s1 == p.G * tiles) {
+    if (key < p.N) {
+      uint16_t* dkr = p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2;
+      uint16_t* dvr = p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int d0 = 32 * db + 16 * hf + 8 * g;
-        if (d0 < D) {
-          f32x16 x = dk[db] * ks_;
-          *reinterpret_cast<u32x4*>(dkr + d0) = pack_b<E>(x, hf);
-          *reinterpret_cast<u32x4*>(dvr + d0) = pack_b<E>(dv[db], hf);
+        for (int hf = 0; hf < 2; ++hf) {
+          const int d0 = 32 * db + 16 * hf + 8 * g;
+          if (d0 < D) {
+            f32x16 x = dk[db] * ks_;
+            *reinterpret_cast<u32x4*>(dkr + d0) = pack_b<E>(x, hf);
+            *reinterpret_cast<u32x4*>(dvr + d0) = pack_b<E>(dv[db], hf);
+          }
         }
-      }
+    }
   } else {
-    float* pr = p.part + (window_slab(p, bhk, kb, piece) * BK + 32 * wave + c) * (2 * D);
+    // Slab 2 wg for a part that starts the run, 2 wg + 1 for one that ends it.
+    const int slab = 2 * wg + (start + s0 == (int64_t)wg * p.chunk ? 0 : 1);
+    float* pr = p.part + ((int64_t)slab * BK + 32 * wave + c) * (2 * D);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -318,28 +409,43 @@ void window_dkdv_kernel(const WindowBwdParams p) {
         }
       }
   }
+  if (p.chunk == 0 || start + s1 >= stop) break;
+  at = start + s1;
+  before += p.G * tiles;
+  // The next block with rows (blocks that no row sees take no tiles).
+  do {
+    if (++kb == p.nkb) {
+      kb = 0;
+      before = 0;
+      ++bhk;
+    }
+    window_tiles(p, kb, tlo, tiles);
+  } while (tiles == 0);
+  }
 }
 
-// dK, dV of the key blocks that were dealt to several workgroups: the sum of
-// their parts, in order.  One thread per 8 elements of keys [0, nkeys) of each
-// KV head: the sinks' blocks, or all of them.
+// Key blocks that were dealt to several workgroups: dK, dV as the sum of their
+// parts, in order; and blocks that no row sees: zeros.  A workgroup per 256 / (D
+// / 8) keys of a block.
 template <class E, int D>
-__global__ __launch_bounds__(256) void window_reduce_kernel(const WindowBwdParams p, int nkeys) {
-  constexpr int CPR = D / 8;
-  const int64_t total = (int64_t)p.B * p.Hk * nkeys * CPR;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int ch = (int)(i % CPR);
-    const int64_t r = i / CPR;
-    const int key = (int)(r % nkeys), bhk = (int)(r / nkeys);
-    const int kb = key / kBwdBlock, pieces = kb < p.sink_blocks ? p.sink_pieces : p.pieces;
-    if (pieces == 1) continue;  // written by its only workgroup
-    const int hk = bhk % p.Hk, b = bhk / p.Hk;
-    const float* src =
-        p.part + (window_slab(p, bhk, kb, 0) * kBwdBlock + key % kBwdBlock) * (2 * D) + 8 * ch;
-    float a[8] = {}, v[8] = {};
+__global__ __launch_bounds__(256) void window_reduce_kernel(const WindowBwdParams p) {
+  constexpr int CPR = D / 8, KEYS = 256 / CPR, PER = kBwdBlock / KEYS;
+  const int sub = (int)(blockIdx.x % PER), item = (int)(blockIdx.x / PER);
+  const int bhk = item / p.nkb, kb = item - bhk * p.nkb;
+  int lo, tiles;
+  window_tiles(p, kb, lo, tiles);
+  const int64_t start = (int64_t)bhk * p.head_tiles + window_before(p, kb);
+  const int64_t w0 = start / p.chunk, w1 = tiles ? (start + (int64_t)p.G * tiles - 1) / p.chunk : w0;
+  if (tiles > 0 && w0 == w1) return;  // written by its only workgroup
+  const int row = sub * KEYS + (int)threadIdx.x / CPR, d0 = 8 * ((int)threadIdx.x % CPR);
+  const int key = kb * kBwdBlock + row;
+  if (key >= p.N) return;
+  float a[8] = {}, v[8] = {};
+  if (tiles > 0) {
 #pragma unroll 4
-    for (int j = 0; j < pieces; ++j, src += kBwdBlock * 2 * D) {
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t slab = 2 * w + (w == w0 && start != w * p.chunk ? 1 : 0);
+      const float* src = p.part + (slab * kBwdBlock + row) * (2 * D) + d0;
       const f32x4 a0 = *reinterpret_cast<const f32x4*>(src);
       const f32x4 a1 = *reinterpret_cast<const f32x4*>(src + 4);
       const f32x4 v0 = *reinterpret_cast<const f32x4*>(src + D);
@@ -352,12 +458,12 @@ __global__ __launch_bounds__(256) void window_reduce_kernel(const WindowBwdParam
         v[4 + e] += v1[e];
       }
     }
-    const int d0 = 8 * ch;
-    *reinterpret_cast<u32x4*>(p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2 + d0) =
-        u32x4{E::pack(a[0], a[1]), E::pack(a[2], a[3]), E::pack(a[4], a[5]), E::pack(a[6], a[7])};
-    *reinterpret_cast<u32x4*>(p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2 + d0) =
-        u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
   }
+  const int hk = bhk % p.Hk, b = bhk / p.Hk;
+  *reinterpret_cast<u32x4*>(p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2 + d0) =
+      u32x4{E::pack(a[0], a[1]), E::pack(a[2], a[3]), E::pack(a[4], a[5]), E::pack(a[6], a[7])};
+  *reinterpret_cast<u32x4*>(p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2 + d0) =
+      u32x4{E::pack(v[0], v[1]), E::pack(v[2], v[3]), E::pack(v[4], v[5]), E::pack(v[6], v[7])};
 }
 
 // ---------------------------------------------------------------- dQ

@@ -45,39 +45,48 @@ fas::RowsSplit fwd_split(const Problem& pr, int64_t window, int64_t sinks) {
                          rows <= fas::kFewRows, false);
 }
 
-// Workgroups per key block of the dK/dV kernel, and its workspace.  A block
-// walks the row tiles (64 rows, G heads) that see it; blocks are cut where they
-// leave CUs idle (one workgroup a CU at D = 128, two below), but not below four
-// tiles, and blocks with sinks, which every later row sees, to about the
-// others' length.
+// How the dK/dV kernel's row tiles (64 rows, G heads) are dealt, and its
+// workspace.  One workgroup a CU runs at D = 128, two below.  Whole key blocks
+// end with the longest, or with whole rounds; equal runs of the list of tiles
+// cost about four tiles a workgroup (K and V again, and parts written) and 8 us
+// for the parts' sum.  The cheaper end is taken.
 struct BwdPlan {
-  int64_t mpad, nkb, sink_blocks = 0, sink_pieces = 1, pieces = 1;
-  size_t nl, delta, part, total;
+  int64_t mpad, nkb, wgs, chunk, head_tiles;
+  size_t delta, part, total;
 };
 BwdPlan bwd_plan(const Problem& pr, int64_t window, int64_t sinks) {
   BwdPlan w{};
-  w.sink_pieces = w.pieces = 1;
   const int64_t bk = fas::kBwdBlock, heads = (int64_t)pr.B * pr.Hk;
   w.mpad = (pr.M + bk - 1) / bk * bk;
   w.nkb = (pr.N + bk - 1) / bk;
-  const int64_t all = (int64_t)pr.G * ((pr.M + 63) / 64);
-  const int64_t tiles = std::min(all, pr.G * ((std::min<int64_t>(window, pr.M) + bk + 63) / 64 + 1));
-  if (tiles < all) w.sink_blocks = (std::min<int64_t>(sinks, pr.N) + bk - 1) / bk;
-  const int64_t n = heads * (w.nkb - w.sink_blocks), slots = pr.D == 128 ? kCus : 2 * kCus;
-  if (n > 0 && n < slots)
-    w.pieces = std::max<int64_t>(1, std::min({(slots + n - 1) / n, tiles / 4, (int64_t)8}));
-  if (w.sink_blocks > 0) {
-    const int64_t len = std::max<int64_t>(4, (tiles + w.pieces - 1) / w.pieces);
-    w.sink_pieces = std::max<int64_t>(1, std::min<int64_t>((all + len - 1) / len, 32));
+  int64_t longest = 0;
+  for (int64_t kb = 0; kb < w.nkb; ++kb) {
+    const int64_t off = (int64_t)pr.N - pr.M, k0 = kb * bk;
+    const int64_t lo = std::max<int64_t>(0, k0 - off) / 64;
+    const int64_t hi = k0 < sinks ? pr.M : std::min<int64_t>(pr.M, k0 + bk - 1 - off + std::min<int64_t>(window, pr.N));
+    const int64_t n = pr.G * std::max<int64_t>(0, (hi + 63) / 64 - lo);
+    longest = std::max(longest, n);
+    w.head_tiles += n;
+  }
+  const int64_t all = heads * w.head_tiles, slots = pr.D == 128 ? kCus : 2 * kCus;
+  const int64_t blocks = heads * w.nkb;
+  w.wgs = blocks;
+  if (all > 0) {
+    const double mean = (double)all / (double)blocks, us_per_tile = pr.D == 128 ? 2.0 : 1.6;
+    const double whole = std::max({(double)longest, (double)all / (double)slots,
+                                   blocks <= slots ? 0.0
+                                                   : mean * (double)((blocks + slots - 1) / slots)});
+    const int64_t chunk = std::max<int64_t>(4, (all + slots - 1) / slots);
+    if ((double)chunk + 4.0 + 8.0 / us_per_tile < whole && chunk < INT_MAX) {
+      w.chunk = chunk;
+      w.wgs = (all + chunk - 1) / chunk;
+      w.wgs = (w.wgs + 7) / 8 * 8;  // an equal number for each XCD; the last may find no tiles
+    }
   }
   const size_t rows = (size_t)pr.B * pr.H * w.mpad * 4;
-  w.nl = 0;
   w.delta = align256(rows);
   w.part = 2 * align256(rows);
-  const size_t slabs =
-      (size_t)heads * ((w.sink_pieces > 1 ? w.sink_blocks * w.sink_pieces : 0) +
-                       (w.pieces > 1 ? (w.nkb - w.sink_blocks) * w.pieces : 0));
-  w.total = w.part + align256(slabs * bk * 2 * pr.D * 4);
+  w.total = w.part + (w.chunk > 0 ? (size_t)w.wgs * 2 * bk * 2 * pr.D * 4 : 0);
   return w;
 }
 
@@ -161,9 +170,9 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   if (pr.M > (1 << 26)) return fail(FAS_ERR_UNSUPPORTED, fn, "seqlen_q exceeds 2^26");
   const BwdPlan w = bwd_plan(pr, window, sinks);
   if ((rc = fas::check_rows_workspace(fn, w.total, ws, ws_bytes))) return rc;
-  const int64_t items = w.sink_blocks * w.sink_pieces + (w.nkb - w.sink_blocks) * w.pieces;
   const int64_t nprep = (w.mpad + (2048 / pr.D) - 1) / (2048 / pr.D);
-  if ((int64_t)pr.B * pr.Hk * items > INT_MAX || (int64_t)pr.B * pr.H * nprep > INT_MAX)
+  if (w.wgs > INT_MAX || (int64_t)pr.B * pr.Hk * w.nkb * 8 > INT_MAX ||
+      (int64_t)pr.B * pr.H * nprep > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more row blocks than one launch takes");
 
   fas::WindowBwdParams p{};
@@ -174,7 +183,7 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   p.dout = static_cast<const uint16_t*>(dout);
   p.lse = lse;
   char* base = static_cast<char*>(ws);
-  p.nl = reinterpret_cast<float*>(base + w.nl);
+  p.nl = reinterpret_cast<float*>(base);
   p.delta = reinterpret_cast<float*>(base + w.delta);
   p.part = reinterpret_cast<float*>(base + w.part);
   p.dq = static_cast<uint16_t*>(dq);
@@ -205,9 +214,9 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   p.nkb = (int)w.nkb;
   p.nrb = (int)(w.mpad / fas::kBwdBlock);
   p.nprep = (int)nprep;
-  p.pieces = (int)w.pieces;
-  p.sink_blocks = (int)w.sink_blocks;
-  p.sink_pieces = (int)w.sink_pieces;
+  p.wgs = (int)w.wgs;
+  p.chunk = (int)w.chunk;
+  p.head_tiles = w.head_tiles;
   p.window = (int)std::min<int64_t>(window, fas::kNoWindow);
   p.sinks = (int)std::min<int64_t>(sinks, fas::kNoWindow);
   p.sm_scale = std::fabs(pr.sm_scale);

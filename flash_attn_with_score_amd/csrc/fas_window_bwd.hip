@@ -11,17 +11,11 @@ static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
     hipLaunchKernelGGL((bwd_prep_kernel<E, D>), dim3((unsigned)(bh * p.nprep)), dim3(256), 0, s,
                        p);
   if (p.N > 0) {
-    const int64_t items = (int64_t)p.sink_blocks * p.sink_pieces +
-                          (int64_t)(p.nkb - p.sink_blocks) * p.pieces;
-    hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)(bhk * items)), dim3(256), 0, s,
-                       p);
-    if (p.pieces > 1 || p.sink_pieces > 1) {
-      const int nkeys = p.pieces > 1 ? p.N : p.sink_blocks * kBwdBlock < p.N
-                                                 ? p.sink_blocks * kBwdBlock : p.N;
-      const int64_t blocks = (bhk * nkeys * (D / 8) + 255) / 256;
-      hipLaunchKernelGGL((window_reduce_kernel<E, D>),
-                         dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, p,
-                         nkeys);
+    hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)p.wgs), dim3(256), 0, s, p);
+    if (p.chunk > 0) {
+      const int per = kBwdBlock * (D / 8) / 256;  // workgroups per key block
+      hipLaunchKernelGGL((window_reduce_kernel<E, D>), dim3((unsigned)(bhk * p.nkb * per)), dim3(256),
+                         0, s, p);
     }
   }
   if (p.M > 0)
