@@ -149,9 +149,128 @@ __device__ __forceinline__ int window_find(const WindowBwdParams& p, int64_t at,
 
 // ---------------------------------------------------------------- dK, dV
 
+// A workgroup's run of the list: block after block, tiles [s0, s1) of each.
+struct WindowRun {
+  int wg, bhk, kb;
+  int tlo, tiles;  // the block's 64-row tiles [tlo, tlo + tiles) of every head
+  int s0, s1;      // of its G * tiles, in head order
+  int64_t at, stop, before, start;  // tiles of the list: the run's, those before the block
+                                    // in its KV head, and the block's first
+  // The run's first block (false: no tiles left for this workgroup).  Runs that
+  // follow each other go to one XCD (workgroup i runs on XCD i % 8): they share
+  // query rows in its L2.
+  __device__ __forceinline__ bool begin(const WindowBwdParams& p) {
+    wg = blockIdx.x;
+    at = stop = before = 0;
+    if (p.chunk > 0) {
+      wg = (wg & 7) * ((int)gridDim.x >> 3) + (wg >> 3);
+      at = (int64_t)wg * p.chunk;
+      stop = min(at + p.chunk, (int64_t)p.B * p.Hk * p.head_tiles);
+      if (at >= stop) return false;
+      bhk = (int)(at / p.head_tiles);
+      kb = window_find(p, at - (int64_t)bhk * p.head_tiles, before);
+    } else {
+      kb = wg / (p.B * p.Hk);  // longest first: blocks with sinks
+      bhk = wg - kb * (p.B * p.Hk);
+    }
+    set(p);
+    return true;
+  }
+  __device__ __forceinline__ void set(const WindowBwdParams& p) {
+    bhk = __builtin_amdgcn_readfirstlane(bhk);
+    kb = __builtin_amdgcn_readfirstlane(kb);
+    window_tiles(p, kb, tlo, tiles);
+    s0 = 0;
+    s1 = p.G * tiles;
+    start = (int64_t)bhk * p.head_tiles + before;
+    if (p.chunk > 0) {
+      s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
+      s1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)s1, stop - start));
+    }
+  }
+  __device__ __forceinline__ bool whole(const WindowBwdParams& p) const {
+    return s0 == 0 && s1 == p.G * tiles;
+  }
+  // The next block with rows (blocks that no row sees take no tiles).
+  __device__ __forceinline__ bool next(const WindowBwdParams& p) {
+    if (p.chunk == 0 || start + s1 >= stop) return false;
+    at = start + s1;
+    before += p.G * tiles;
+    do {
+      if (++kb == p.nkb) {
+        kb = 0;
+        before = 0;
+        ++bhk;
+      }
+      window_tiles(p, kb, tlo, tiles);
+    } while (tiles == 0);
+    set(p);
+    return true;
+  }
+  // Slab of this workgroup's part: 2 wg where it starts the run, else 2 wg + 1.
+  __device__ __forceinline__ int slab(const WindowBwdParams& p) const {
+    return 2 * wg + (start + s0 == (int64_t)wg * p.chunk ? 0 : 1);
+  }
+};
+
+// Which keys of the wave's 32, from key0 on, a run of 32 rows sees, from
+// position p0 on: some of them, all of them; and per lane (key key0 + c) the
+// row position - key below which it does (a key past N: never).
+struct WindowSight {
+  int key0, N, window, sinks;
+  __device__ __forceinline__ bool live(int p0) const {
+    return p0 + 31 >= key0 && (key0 + 31 > p0 - window || key0 < sinks);
+  }
+  __device__ __forceinline__ bool full(int p0) const {
+    return p0 >= key0 + 31 && key0 + 31 < N && (key0 > p0 + 31 - window || key0 + 32 <= sinks);
+  }
+  __device__ __forceinline__ int reach(int c) const {
+    return key0 + c >= N ? 0 : key0 + c < sinks ? 0x7fffffff : window;
+  }
+};
+
+// dV^T (dv) or dK^T of the wave's keys, register r of block db: key `key`, head
+// dim 32 db + acc_row(r, g): to its place, or into the part's slab.
+template <class E, int D, int DB>
+__device__ __forceinline__ void window_store(const WindowBwdParams& p, const WindowRun& run, bool dv,
+                                             const f32x16 (&acc)[DB], int key, int g) {
+  const int b = run.bhk / p.Hk, hk = run.bhk - b * p.Hk;
+  const float scale = dv ? 1.f : p.scale_signed;
+  if (run.whole(p)) {
+    if (key >= p.N) return;
+    uint16_t* out = dv ? p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2
+                       : p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int d0 = 32 * db + 16 * hf + 8 * g;
+        if (d0 < D) *reinterpret_cast<u32x4*>(out + d0) = pack_b<E>(acc[db] * scale, hf);
+      }
+    return;
+  }
+  float* out = p.part + ((int64_t)run.slab(p) * kBwdBlock + key % kBwdBlock) * (2 * D) + (dv ? D : 0);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int d0 = 32 * db + 16 * hf + 8 * g;
+      if (d0 < D) {
+        const f32x16 x = acc[db] * scale;
+        const int r = 8 * hf;
+        *reinterpret_cast<f32x4*>(out + d0) = f32x4{x[r], x[r + 1], x[r + 2], x[r + 3]};
+        *reinterpret_cast<f32x4*>(out + d0 + 4) = f32x4{x[r + 4], x[r + 5], x[r + 6], x[r + 7]};
+      }
+    }
+}
+
+// dK, dV up to D = 64: four waves, each with both products of its 32 keys; two
+// workgroups a CU cover each other's waits (the split of the work between two
+// waves that window_dkdv_kernel makes costs them more than it gives, their LDS
+// holding one workgroup a CU: B1 H32 S8192 D64 window 1024, backward, 401 / 477 us).
 template <class E, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 2 : 1)))
-void window_dkdv_kernel(const WindowBwdParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void window_dkdv_small_kernel(const WindowBwdParams p) {
   constexpr int KS = D / 16;
   constexpr int DB = D >= 32 ? D / 32 : 1;
   constexpr int NW = 4;
@@ -167,261 +286,392 @@ void window_dkdv_kernel(const WindowBwdParams p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, c = lane & 31, g = lane >> 5;
-  // Runs of the list that follow each other go to one XCD (workgroup i runs on
-  // XCD i % 8): they share query rows in its L2.
-  int wg = blockIdx.x;
-  if (gridDim.x % 8 == 0) wg = (wg & 7) * ((int)gridDim.x >> 3) + (wg >> 3);
-  int64_t at = 0, stop = 0, before = 0;  // tiles of the list; those before block kb of this KV head
-  int bhk, kb;
-  if (p.chunk > 0) {
-    at = (int64_t)wg * p.chunk;
-    stop = min(at + p.chunk, (int64_t)p.B * p.Hk * p.head_tiles);
-    if (at >= stop) return;
-    bhk = (int)(at / p.head_tiles);
-    kb = window_find(p, at - (int64_t)bhk * p.head_tiles, before);
-  } else {
-    wg = blockIdx.x;  // longest first: blocks with sinks
-    kb = wg / (p.B * p.Hk);
-    bhk = wg - kb * (p.B * p.Hk);
-  }
+  WindowRun run;
+  if (!run.begin(p)) return;
   const float qk = p.qk_scale;
   const uint32_t q_base = lds_addr(&qlds[0][0]), g_base = lds_addr(&glds[0][0]);
   const TileDma<D> qdma(wave, lane, (uint32_t)p.sq2), gdma(wave, lane, (uint32_t)p.sg2);
 
-  for (;;) {  // one key block, or the part of it in this workgroup's run
-  bhk = __builtin_amdgcn_readfirstlane(bhk);
-  kb = __builtin_amdgcn_readfirstlane(kb);
-  int tlo, tiles;
-  window_tiles(p, kb, tlo, tiles);
-  // Tiles [s0, s1) of the block's G * tiles, in head order.
-  int s0 = 0, s1 = p.G * tiles;
-  const int64_t start = (int64_t)bhk * p.head_tiles + before;  // the block's first in the list
-  if (p.chunk > 0) {
-    s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
-    s1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)s1, stop - start));
-  }
-  const int b = bhk / p.Hk, hk = bhk % p.Hk;
-  const int h0 = hk * p.G;
-  const int key0 = kb * BK + 32 * wave;  // this wave's keys [key0, key0 + 32)
+  do {  // one key block, or the part of it in this workgroup's run
+    const int b = run.bhk / p.Hk, hk = run.bhk % p.Hk;
+    const int h0 = hk * p.G;
+    const int key0 = run.kb * BK + 32 * wave;  // this wave's keys [key0, key0 + 32)
+    const WindowSight sight{key0, p.N, p.window, p.sinks};
+    const int reach = sight.reach(c), tlo = run.tlo, tiles = run.tiles;
 
-  const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
-  const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
-  u32x4 kreg[KS], vreg[KS];
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes);
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
+    u32x4 kreg[KS], vreg[KS];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    kreg[ks] = buf_load16(rk, (uint32_t)(((key0 + c) * p.sk2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
-    vreg[ks] = buf_load16(rv, (uint32_t)(((key0 + c) * p.sv2 + 16 * ks + 8 * g) * 2));
-  }
+    for (int ks = 0; ks < KS; ++ks) {
+      kreg[ks] = buf_load16(rk, (uint32_t)(((key0 + c) * p.sk2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
+      vreg[ks] = buf_load16(rv, (uint32_t)(((key0 + c) * p.sv2 + 16 * ks + 8 * g) * 2));
+    }
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kreg[ks]), "+v"(vreg[ks]));
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kreg[ks]), "+v"(vreg[ks]));
 
-  f32x16 dk[DB], dv[DB];
+    f32x16 dk[DB], dv[DB];
 #pragma unroll
-  for (int db = 0; db < DB; ++db) {
-    dk[db] = f32x16{};
-    dv[db] = f32x16{};
-  }
+    for (int db = 0; db < DB; ++db) {
+      dk[db] = f32x16{};
+      dv[db] = f32x16{};
+    }
 
-  // Row position - key, per lane: a row sees key key0 + c iff 0 <= difference
-  // < reach (a key past N: never).
+    const VtOff vto = vt_offsets<D>(lane);
+    const uint32_t rco = row_chunk_offset<D>(perm_row(c), g);
+
+    for (int hh = 0; hh < p.G; ++hh) {
+      const int t0 = tlo + max(0, run.s0 - hh * tiles), t1 = tlo + min(tiles, run.s1 - hh * tiles);
+      if (t0 >= t1) continue;
+      const int h = h0 + hh;
+      const int64_t bh = (int64_t)b * p.H + h;
+      const i32x4 wq = make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes);
+      const i32x4 wg = make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
+      const float* nlg = p.nl + bh * p.Mpad;
+      const float* xg = p.delta + bh * p.Mpad;
+      float nst = 0.f, xst = 0.f;
+      auto fetch = [&](int t, int s) __attribute__((always_inline)) {
+        qdma.fetch(wq, t * TQ, 0, 0, q_base + (uint32_t)(s * TILE * 2));
+        gdma.fetch(wg, t * TQ, 0, 0, g_base + (uint32_t)(s * TILE * 2));
+        if (tid < TQ) {
+          nst = nlg[t * TQ + tid];
+          xst = xg[t * TQ + tid];
+        }
+      };
+      auto stash = [&](int s) __attribute__((always_inline)) {
+        if (tid < TQ) {
+          nlds[s][tid] = nst;
+          xlds[s][tid] = xst;
+        }
+      };
+      fetch(t0, 0);
+      vm_wait_all();
+      stash(0);
+      __syncthreads();
+      auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
+        constexpr int stage = decltype(stage_tag)::value;
+        const bool more = t + 1 < t1;
+        if (more) fetch(t + 1, stage ^ 1);
+        const uint16_t* qt = qlds[stage];
+        const uint16_t* gt = glds[stage];
+        // One 32-row block; masked and unmasked copies of the elementwise part
+        // join before the dV / dK products.
+        auto body = [&](int qb, bool full) __attribute__((always_inline)) {
+          const int r0 = t * TQ + 32 * qb;
+          // Register r holds query row r0 + acc_row(r, g) and key key0 + c.
+          // Operand fetches go two k-steps ahead of the products that take them,
+          // and S and dP alternate.
+          __builtin_amdgcn_sched_barrier(0);
+          uint32_t ro = rco;
+          opaque(ro);
+          f32x16 s = f32x16{}, dp, nl;
+          load8(dp, &xlds[stage][32 * qb + 8 * g], 0, 0);
+          load8(dp, &xlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+          u32x4 aq[KS], ag[KS];
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            aq[ks] = lds_row_chunk(qt + 32 * qb * D, ro, ks);
+            ag[ks] = lds_row_chunk(gt + 32 * qb * D, ro, ks);
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            s = E::mma(aq[ks], kreg[ks], s);
+            dp = E::mma(ag[ks], vreg[ks], dp);
+          }
+          load8(nl, &nlds[stage][32 * qb + 8 * g], 0, 0);
+          load8(nl, &nlds[stage][32 * qb + 16 + 8 * g], 0, 1);
+          {
+            constexpr int PD = KS < 3 ? KS : 3;
+            __builtin_amdgcn_sched_group_barrier(0x100, 4 + 2 * PD, 0);  // DS read
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
+              if (i + PD < KS)
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+              else if (i + PD == KS)
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          VtOff vo = vto;
+          opaque(vo);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = exp2f_fast(fmaf(s[r], qk, nl[r]));
+          if (!full) {
+            int diff = p.causal_off + r0 - (key0 + c);
+            asm volatile("" : "+v"(diff));  // (a branch, not 32 selects on every block)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if ((uint32_t)(diff + acc_row(r, g)) >= (uint32_t)reach) s[r] = 0.f;
+          }
+          u32x4 tg[2 * DB], tq[2 * DB];
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              tg[2 * db + h] = lds_vt_operand<D>(gt, vo, db, 2 * qb + h);
+              tq[2 * db + h] = lds_vt_operand<D>(qt, vo, db, 2 * qb + h);
+            }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+          const u32x4 pb[2] = {pack_b<E>(s, 0), pack_b<E>(s, 1)};
+          const u32x4 sb[2] = {pack_b<E>(dp, 0), pack_b<E>(dp, 1)};
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              dv[db] = E::mma(tg[2 * db + h], pb[h], dv[db]);
+              dk[db] = E::mma(tq[2 * db + h], sb[h], dk[db]);
+            }
+          {
+            constexpr int PD = 2;  // operand pairs ahead
+            __builtin_amdgcn_sched_group_barrier(0x100, 4 * PD, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * DB; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+              if (i + PD < 2 * DB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            }
+          }
+        };
+        const int p0 = p.causal_off + t * TQ;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb)
+          if (sight.live(p0 + 32 * qb)) body(qb, sight.full(p0 + 32 * qb));
+        if (more) {
+          vm_wait_all();
+          stash(stage ^ 1);
+        }
+        __syncthreads();
+      };
+      for (int t = t0; t < t1; t += 2) {
+        step(t, std::integral_constant<int, 0>{});
+        if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
+      }
+    }
+
+    window_store<E, D>(p, run, false, dk, key0 + c, g);
+    window_store<E, D>(p, run, true, dv, key0 + c, g);
+  } while (run.next(p));
+}
+
+// dK, dV: eight waves, two for each 32 keys of the block: one turns S into P and
+// accumulates dV, the other turns dP into dS and accumulates dK, a tile later,
+// with the P that the first left in LDS.  Each does half the products and holds
+// half the accumulators, so two waves a SIMD fit (one that did both took 350
+// registers), and one's exponentials and waits run beside the other's products
+// (B1 H32/8 S4096 D128 window 1024: 204 us, with
+// one wave a SIMD for both 212).  P passes in fp16 whatever the input
+// type: within 2^-12 of its value, and 2^-25 below fp16's normal range, both
+// beside the rounding of dS itself.
+template <int D>
+struct WindowDkdvLds {
+  uint16_t q[3][64 * D], g[3][64 * D];  // Q and dO
+  u32x4 p[2][4][2][2][64];              // P of two tiles: key wave, 32-row block, half, lane
+  float nl[3][64], x[3][64];            // -L log2(e), -delta
+};
+// One role (FIRST: S, P, dV; else dP, dS, dK), in code of its own: where the two
+// shared a loop their accumulators were moved at every join.
+template <class E, int D, bool first>
+__device__ __forceinline__ void window_dkdv(const WindowBwdParams& p, WindowDkdvLds<D>& lds) {
+  constexpr int KS = D / 16;
+  constexpr int DB = D >= 32 ? D / 32 : 1;
+  constexpr int BK = kBwdBlock;  // keys per workgroup
+  constexpr int TQ = 64;         // query rows per tile
+  constexpr int TILE = TQ * D;
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, c = lane & 31, g = lane >> 5;
+  const int kw = wave & 3;
+  WindowRun run;
+  if (!run.begin(p)) return;
+  const float qk = p.qk_scale;
+  // The first waves fetch Q, the second ones dO.
+  const TileDma<D> dma(kw, lane, (uint32_t)(first ? p.sq2 : p.sg2));
+  const uint32_t dma_base = lds_addr(first ? &lds.q[0][0] : &lds.g[0][0]);
   const VtOff vto = vt_offsets<D>(lane);
   const uint32_t rco = row_chunk_offset<D>(perm_row(c), g);
-  const int reach = key0 + c >= p.N ? 0 : key0 + c < p.sinks ? 0x7fffffff : p.window;
 
-  for (int hh = 0; hh < p.G; ++hh) {
-    const int t0 = tlo + max(0, s0 - hh * tiles), t1 = tlo + min(tiles, s1 - hh * tiles);
-    if (t0 >= t1) continue;
-    const int h = h0 + hh;
-    const int64_t bh = (int64_t)b * p.H + h;
-    const i32x4 wq = make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes);
-    const i32x4 wg = make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
-    const float* nlg = p.nl + bh * p.Mpad;
-    const float* xg = p.delta + bh * p.Mpad;
-    float nst = 0.f, xst = 0.f;
-    auto fetch = [&](int t, int s) __attribute__((always_inline)) {
-      qdma.fetch(wq, t * TQ, 0, 0, q_base + (uint32_t)(s * TILE * 2));
-      gdma.fetch(wg, t * TQ, 0, 0, g_base + (uint32_t)(s * TILE * 2));
-      if (tid < TQ) {
-        nst = nlg[t * TQ + tid];
-        xst = xg[t * TQ + tid];
+  do {  // one key block, or the part of it in this workgroup's run
+    const int b = __builtin_amdgcn_readfirstlane(run.bhk / p.Hk), hk = run.bhk - b * p.Hk;
+    const int h0 = hk * p.G;
+    const int key0 = run.kb * BK + 32 * kw;  // this wave's keys [key0, key0 + 32)
+    const WindowSight sight{key0, p.N, p.window, p.sinks};
+    const int reach = sight.reach(c);
+
+    // K or V (B operand of S = Q K^T or dP = dO V^T): lane holds row key0 + c.
+    // K carries the sign of a negative sm_scale.
+    u32x4 kv[KS];
+    {
+      const __amdgpu_buffer_rsrc_t r =
+          first ? make_rsrc(p.k + b * p.sk0 + hk * p.sk1, p.k_bytes)
+                : make_rsrc(p.v + b * p.sv0 + hk * p.sv1, p.v_bytes);
+      const int64_t stride = first ? p.sk2 : p.sv2;
+      const uint32_t flip = first ? p.qneg : 0u;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        kv[ks] = buf_load16(r, (uint32_t)(((key0 + c) * stride + 16 * ks + 8 * g) * 2)) ^ flip;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kv[ks]));
+    }
+    f32x16 acc[DB];  // dV^T or dK^T
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+    // Tile `t` of head h0 + hh on its way to stage st; its row values into a
+    // register of the waves' first (nl) and fifth (-delta).
+    float rv = 0.f;
+    auto fetch = [&](int hh, int t, int st) __attribute__((always_inline)) {
+      const int h = h0 + hh;
+      const i32x4 r = first ? make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes)
+                            : make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
+      dma.fetch(r, t * TQ, 0, 0, dma_base + (uint32_t)(st * TILE * 2));
+      if (kw == 0) {
+        const int64_t row = ((int64_t)b * p.H + h) * p.Mpad + t * TQ + lane;
+        rv = first ? p.nl[row] : p.delta[row];
       }
     };
-    auto stash = [&](int s) __attribute__((always_inline)) {
-      if (tid < TQ) {
-        nlds[s][tid] = nst;
-        xlds[s][tid] = xst;
+    auto land = [&](int st) __attribute__((always_inline)) {
+      vm_wait_all();
+      if (kw == 0) (first ? lds.nl[st] : lds.x[st])[lane] = rv;
+    };
+    // One product pair's schedule: operand fetches two k-steps (pairs) ahead.
+    auto row_products = [&](const uint16_t* tile, f32x16 x) __attribute__((always_inline)) {
+      uint32_t ro = rco;
+      opaque(ro);
+      u32x4 a[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) a[ks] = lds_row_chunk(tile, ro, ks);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) x = E::mma(a[ks], kv[ks], x);
+      return x;
+    };
+    auto col_products = [&](const uint16_t* tile, int qb, const u32x4 (&w)[2])
+                            __attribute__((always_inline)) {
+      VtOff vo = vto;
+      opaque(vo);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          acc[db] = E::mma(lds_vt_operand<D>(tile, vo, db, 2 * qb + h), w[h], acc[db]);
+    };
+    auto sched_rows = [&]() __attribute__((always_inline)) {
+      constexpr int PD = KS < 4 ? KS : 4;
+      __builtin_amdgcn_sched_group_barrier(0x100, 4 + PD, 0);  // DS read
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        if (i + PD < KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
     };
-    fetch(t0, 0);
-    vm_wait_all();
-    stash(0);
-    __syncthreads();
-    auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
-      constexpr int stage = decltype(stage_tag)::value;
-      const bool more = t + 1 < t1;
-      if (more) fetch(t + 1, stage ^ 1);
-      const uint16_t* qt = qlds[stage];
-      const uint16_t* gt = glds[stage];
-      // One 32-row block; masked and unmasked copies of the elementwise part
-      // join before the dV / dK products.
-      auto body = [&](int qb, bool full) __attribute__((always_inline)) {
-        const int r0 = t * TQ + 32 * qb;
-        // Register r holds query row r0 + acc_row(r, g) and key key0 + c.  One
-        // wave a SIMD runs at D = 128, so nothing covers the wait for an
-        // operand: fetches go two k-steps ahead of the products that take
-        // them, and S and dP alternate.
+    auto sched_cols = [&]() __attribute__((always_inline)) {
+      constexpr int PD = 2 * DB < 3 ? 2 * DB : 3;
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * PD, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + PD < 2 * DB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+    };
+    // P of a 32-row block (register r: query row acc_row(r, g), key key0 + c).
+    auto weights = [&](int st, int buf, int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const int p0 = p.causal_off + t * TQ + 32 * qb;
+        if (!sight.live(p0)) continue;
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t ro = rco;
-        opaque(ro);
-        f32x16 s = f32x16{}, dp, nl;
-        load8(dp, &xlds[stage][32 * qb + 8 * g], 0, 0);
-        load8(dp, &xlds[stage][32 * qb + 16 + 8 * g], 0, 1);
-        u32x4 aq[KS], ag[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          aq[ks] = lds_row_chunk(qt + 32 * qb * D, ro, ks);
-          ag[ks] = lds_row_chunk(gt + 32 * qb * D, ro, ks);
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          s = E::mma(aq[ks], kreg[ks], s);
-          dp = E::mma(ag[ks], vreg[ks], dp);
-        }
-        load8(nl, &nlds[stage][32 * qb + 8 * g], 0, 0);
-        load8(nl, &nlds[stage][32 * qb + 16 + 8 * g], 0, 1);
-        {
-          constexpr int PD = KS < 3 ? KS : 3;
-          __builtin_amdgcn_sched_group_barrier(0x100, 4 + 2 * PD, 0);  // DS read
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // MFMA
-            if (i + PD < KS)
-              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            else if (i + PD == KS)
-              __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-          }
-        }
+        f32x16 nl;
+        load8(nl, &lds.nl[st][32 * qb + 8 * g], 0, 0);
+        load8(nl, &lds.nl[st][32 * qb + 16 + 8 * g], 0, 1);
+        f32x16 s = row_products(&lds.q[st][32 * qb * D], f32x16{});
+        sched_rows();
         __builtin_amdgcn_sched_barrier(0);
-        VtOff vo = vto;
-        opaque(vo);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = exp2f_fast(fmaf(s[r], qk, nl[r]));
-        if (!full) {
-          int diff = p.causal_off + r0 - (key0 + c);
+        if (!sight.full(p0)) {
+          int diff = p0 - (key0 + c);
           asm volatile("" : "+v"(diff));  // (a branch, not 32 selects on every block)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if ((uint32_t)(diff + acc_row(r, g)) >= (uint32_t)reach) s[r] = 0.f;
         }
-        u32x4 tg[2 * DB], tq[2 * DB];
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            tg[2 * db + h] = lds_vt_operand<D>(gt, vo, db, 2 * qb + h);
-            tq[2 * db + h] = lds_vt_operand<D>(qt, vo, db, 2 * qb + h);
-          }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] *= s[r];
         const u32x4 pb[2] = {pack_b<E>(s, 0), pack_b<E>(s, 1)};
-        const u32x4 sb[2] = {pack_b<E>(dp, 0), pack_b<E>(dp, 1)};
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            dv[db] = E::mma(tg[2 * db + h], pb[h], dv[db]);
-            dk[db] = E::mma(tq[2 * db + h], sb[h], dk[db]);
-          }
-        {
-          constexpr int PD = 2;  // operand pairs ahead
-          __builtin_amdgcn_sched_group_barrier(0x100, 4 * PD, 0);
-#pragma unroll
-          for (int i = 0; i < 2 * DB; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-            if (i + PD < 2 * DB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-          }
-        }
-      };
-      // Positions p0 .. p0 + 31 against the wave's keys.
-      auto live = [&](int p0) {
-        return p0 + 31 >= key0 && (key0 + 31 > p0 - p.window || key0 < p.sinks);
-      };
-      auto full = [&](int p0) {
-        return p0 >= key0 + 31 && key0 + 31 < p.N &&
-               (key0 > p0 + 31 - p.window || key0 + 32 <= p.sinks);
-      };
-      const int p0 = p.causal_off + t * TQ;
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb)
-        if (live(p0 + 32 * qb)) body(qb, full(p0 + 32 * qb));
-      if (more) {
-        vm_wait_all();
-        stash(stage ^ 1);
+        for (int h = 0; h < 2; ++h) lds.p[buf][kw][qb][h][lane] = pack_b<F16>(s, h);
+        col_products(lds.g[st], qb, pb);
+        sched_cols();
       }
-      __syncthreads();
     };
-    for (int t = t0; t < t1; t += 2) {
-      step(t, std::integral_constant<int, 0>{});
-      if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
-    }
-  }
-
-  // Lane (c, g), register r of block db: key key0 + c, head dim
-  // 32db + acc_row(r, g).
-  const int key = key0 + c;
-  const float ks_ = p.scale_signed;
-  if (s0 == 0 && s1 == p.G * tiles) {
-    if (key < p.N) {
-      uint16_t* dkr = p.dk + b * p.sdk0 + hk * p.sdk1 + (int64_t)key * p.sdk2;
-      uint16_t* dvr = p.dv + b * p.sdv0 + hk * p.sdv1 + (int64_t)key * p.sdv2;
+    auto grads = [&](int st, int buf, int t) __attribute__((always_inline)) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+      for (int qb = 0; qb < 2; ++qb) {
+        const int p0 = p.causal_off + t * TQ + 32 * qb;
+        if (!sight.live(p0)) continue;
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 dp;
+        load8(dp, &lds.x[st][32 * qb + 8 * g], 0, 0);
+        load8(dp, &lds.x[st][32 * qb + 16 + 8 * g], 0, 1);
+        dp = row_products(&lds.g[st][32 * qb * D], dp);
+        sched_rows();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int d0 = 32 * db + 16 * hf + 8 * g;
-          if (d0 < D) {
-            f32x16 x = dk[db] * ks_;
-            *reinterpret_cast<u32x4*>(dkr + d0) = pack_b<E>(x, hf);
-            *reinterpret_cast<u32x4*>(dvr + d0) = pack_b<E>(dv[db], hf);
-          }
+        for (int h = 0; h < 2; ++h) {
+          float w[8];
+          unpack8<F16>(lds.p[buf][kw][qb][h][lane], w);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) dp[8 * h + r] *= w[r];
         }
-    }
-  } else {
-    // Slab 2 wg for a part that starts the run, 2 wg + 1 for one that ends it.
-    const int slab = 2 * wg + (start + s0 == (int64_t)wg * p.chunk ? 0 : 1);
-    float* pr = p.part + ((int64_t)slab * BK + 32 * wave + c) * (2 * D);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int d0 = 32 * db + 16 * hf + 8 * g;
-        if (d0 < D) {
-          const f32x16& x = dk[db];
-          const f32x16& y = dv[db];
-          const int r = 8 * hf;
-          *reinterpret_cast<f32x4*>(pr + d0) =
-              f32x4{x[r] * ks_, x[r + 1] * ks_, x[r + 2] * ks_, x[r + 3] * ks_};
-          *reinterpret_cast<f32x4*>(pr + d0 + 4) =
-              f32x4{x[r + 4] * ks_, x[r + 5] * ks_, x[r + 6] * ks_, x[r + 7] * ks_};
-          *reinterpret_cast<f32x4*>(pr + D + d0) = f32x4{y[r], y[r + 1], y[r + 2], y[r + 3]};
-          *reinterpret_cast<f32x4*>(pr + D + d0 + 4) =
-              f32x4{y[r + 4], y[r + 5], y[r + 6], y[r + 7]};
-        }
+        const u32x4 sb[2] = {pack_b<E>(dp, 0), pack_b<E>(dp, 1)};
+        col_products(lds.q[st], qb, sb);
+        sched_cols();
       }
-  }
-  if (p.chunk == 0 || start + s1 >= stop) break;
-  at = start + s1;
-  before += p.G * tiles;
-  // The next block with rows (blocks that no row sees take no tiles).
-  do {
-    if (++kb == p.nkb) {
-      kb = 0;
-      before = 0;
-      ++bhk;
+    };
+
+    // Step i: the first waves take tile i, the second ones tile i - 1, while tile
+    // i + 1 arrives: three stages, two buffers of P.
+    const int n = run.s1 - run.s0;
+    int hh = n > 0 ? run.s0 / run.tiles : 0, tt = run.s0 - hh * run.tiles;  // the tile to fetch next
+    int t_prev = 0, t_cur = run.tlo + tt, t_next;
+    if (n > 0) {
+      fetch(hh, run.tlo + tt, 0);
+      land(0);
     }
-    window_tiles(p, kb, tlo, tiles);
-  } while (tiles == 0);
-  }
+    lds_barrier();
+    int st_prev = 2, st_cur = 0, st_next = 1;
+    for (int i = 0; i <= n && n > 0; ++i) {
+      if (++tt == run.tiles) {
+        tt = 0;
+        ++hh;
+      }
+      t_next = run.tlo + tt;
+      const bool more = i + 1 < n;
+      if (more) fetch(hh, t_next, st_next);
+      if constexpr (first) {
+        if (i < n) weights(st_cur, i & 1, t_cur);
+      } else {
+        if (i > 0) grads(st_prev, (i & 1) ^ 1, t_prev);
+      }
+      if (more) land(st_next);
+      lds_barrier();
+      t_prev = t_cur;
+      t_cur = t_next;
+      const int s = st_prev;
+      st_prev = st_cur;
+      st_cur = st_next;
+      st_next = s;
+    }
+
+    window_store<E, D>(p, run, first, acc, key0 + c, g);
+  } while (run.next(p));
+}
+template <class E, int D>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+void window_dkdv_kernel(const WindowBwdParams p) {
+  __shared__ __attribute__((aligned(16))) WindowDkdvLds<D> lds;
+  if (__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) < 4)
+    window_dkdv<E, D, true>(p, lds);
+  else
+    window_dkdv<E, D, false>(p, lds);
 }
 
 // Key blocks that were dealt to several workgroups: dK, dV as the sum of their

@@ -11,7 +11,11 @@ static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
     hipLaunchKernelGGL((bwd_prep_kernel<E, D>), dim3((unsigned)(bh * p.nprep)), dim3(256), 0, s,
                        p);
   if (p.N > 0) {
-    hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)p.wgs), dim3(256), 0, s, p);
+    if constexpr (D == 128)
+      hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)p.wgs), dim3(512), 0, s, p);
+    else
+      hipLaunchKernelGGL((window_dkdv_small_kernel<E, D>), dim3((unsigned)p.wgs), dim3(256), 0, s,
+                         p);
     if (p.chunk > 0) {
       const int per = kBwdBlock * (D / 8) / 256;  // workgroups per key block
       hipLaunchKernelGGL((window_reduce_kernel<E, D>), dim3((unsigned)(bhk * p.nkb * per)), dim3(256),

@@ -28,7 +28,9 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None) -> d
     dP - delta: D products each, delta from the rounded out:
       u = 2 (D + 2) f sum |do||v| + (D + 2) f sum |do||out| + sum |do| out_bound
     (u per pair), and dS = P (dP - delta), rounded for its products:
-      e = P u + |dS| (half + 2 w + 4 f).
+      e = P u + |dS| (half + 2 w + 4 f);
+    for dk P may pass between waves in fp16 (half a step: 2^-12 of its value, 2^-25
+    at least):  e + |dS| 2^-12 + |dP - delta| 2^-25 where the pair is visible.
     dq: half |dq| + s sum_j (e + 2 N f |dS|) |k|;  dk alike over rows."""
     Hq, M, D = q.shape
     Hk, N = k.shape[:2]
@@ -65,6 +67,8 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None) -> d
         * fold(P.transpose(1, 2) @ do.abs())
     res["dq_bound"] = half * res["dq"].abs() + tiny + (1 + half) * abs(scale) \
         * ((e + 2 * N * f * dS.abs()) @ kx.abs())
+    e = e + dS.abs() * 2.0 ** -12 + torch.where(see, 2.0 ** -25, 0.0) \
+        * (dP - (do * out).sum(-1, keepdim=True)).abs()
     res["dk_bound"] = half * res["dk"].abs() + tiny + (1 + half) * abs(scale) \
         * fold((e + 2 * M * G * f * dS.abs()).transpose(1, 2) @ q.abs())
     return res
