@@ -369,6 +369,7 @@ constexpr int kNoWindow = 1 << 30;
 // parts of key blocks, slabs of 128 keys x 2D, two for each workgroup of the
 // dK/dV kernel.
 struct WindowBwdParams : BwdParams {
+  uint32_t o_bytes;    // extent of a head's rows of o
   int window, sinks;
   int wgs;             // workgroups of the dK/dV kernel
   int chunk;           // row tiles of each, or 0: a whole key block each

@@ -2,10 +2,13 @@
 // of fas_rows.hpp with DenseSource and DenseFewSource) and backward.
 //
 // Query row i is at position p = (N - M) + i and sees key j iff j <= p and
-// (j > p - window or j < sinks).  The backward has attention()'s three passes
+// (j > p - window or j < sinks).  The backward has attention()'s products
 // (fas_bwd.hpp: the operand layouts) over the visible pairs alone:
 //
-//   bwd_prep_kernel       per row: -delta = -sum_d O dO and -L log2(e)
+//   window_dq_kernel      query-block outer, over tiles of 64 entries of the key
+//                         list that RowsPlan describes: S^T, P^T, dS^T,
+//                         dQ^T += K^T dS^T.  It first forms its rows' delta and
+//                         exponent offsets and leaves them for the next kernel.
 //   window_dkdv_kernel    key-block outer: S, P, dP, dS, dV^T += dO^T P,
 //                         dK^T += Q^T dS.  The rows that see a block of 128
 //                         keys are one run: those at most `window` behind its
@@ -18,9 +21,6 @@
 //                         slabs, two a workgroup, that window_reduce_kernel
 //                         adds in order.  Where whole blocks are even enough
 //                         (p.chunk 0) a workgroup takes one.
-//   window_dq_kernel      query-block outer, over tiles of 64 entries of the key
-//                         list that RowsPlan describes: S^T, P^T, dS^T,
-//                         dQ^T += K^T dS^T.
 //
 // A pair that a row does not see has P = 0 and so dS = 0; P and dS are rounded
 // to the input type for their products, everything else is fp32.
@@ -748,9 +748,35 @@ void window_dq_kernel(const WindowBwdParams p) {
     qreg[ks] = buf_load16(rq, (uint32_t)((qrow * p.sq2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
     greg[ks] = buf_load16(rg, (uint32_t)((qrow * p.sg2 + 16 * ks + 8 * g) * 2));
   }
-  // Rows past M read nl = -inf (padding), so their P is 0.
-  const float nl = p.nl[(int64_t)bh * p.Mpad + qrow];
-  const float xl = p.delta[(int64_t)bh * p.Mpad + qrow];
+  // The row's -delta = -sum_d O dO and nl = -L log2(e), the base-2 exponent offset
+  // of its weights (-inf, so that P is 0, for rows that see no key and for the
+  // padding past M), here and for the dK/dV kernel, which runs next.  (A pass of
+  // its own over O and dO took 14 us of 339 at B1 H32/8 S4096 D128.)
+  float nl = neg_inf(), xl = 0.f;
+  {
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc(p.o + b * p.so0 + h * p.so1, p.o_bytes);
+    u32x4 oreg[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      oreg[ks] = buf_load16(ro, (uint32_t)((qrow * p.so2 + 16 * ks + 8 * g) * 2));
+    if (qrow < p.M) {
+      const float L = p.lse[b * p.sl0 + h * p.sl1 + (int64_t)qrow * p.sl2];
+      if (L != neg_inf()) nl = -L * kLog2e;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float x[8], y[8];
+      unpack8<E>(oreg[ks], x);
+      unpack8<E>(greg[ks], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) xl = fmaf(x[e], y[e], xl);
+    }
+    xl = -xor32_add(xl);
+    if (g == 0) {
+      p.nl[(int64_t)bh * p.Mpad + qrow] = nl;
+      p.delta[(int64_t)bh * p.Mpad + qrow] = xl;
+    }
+  }
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]), "+v"(greg[ks]));
 

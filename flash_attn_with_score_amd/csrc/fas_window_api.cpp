@@ -170,9 +170,8 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   if (pr.M > (1 << 26)) return fail(FAS_ERR_UNSUPPORTED, fn, "seqlen_q exceeds 2^26");
   const BwdPlan w = bwd_plan(pr, window, sinks);
   if ((rc = fas::check_rows_workspace(fn, w.total, ws, ws_bytes))) return rc;
-  const int64_t nprep = (w.mpad + (2048 / pr.D) - 1) / (2048 / pr.D);
   if (w.wgs > INT_MAX || (int64_t)pr.B * pr.Hk * w.nkb * 8 > INT_MAX ||
-      (int64_t)pr.B * pr.H * nprep > INT_MAX)
+      (int64_t)pr.B * pr.H * (w.mpad / fas::kBwdBlock) > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more row blocks than one launch takes");
 
   fas::WindowBwdParams p{};
@@ -199,6 +198,7 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
     p.sl0 = lst[0]; p.sl1 = lst[1]; p.sl2 = lst[2];
     p.q_bytes = slice_bytes(pr.M, p.sq2, pr.D);
     p.g_bytes = slice_bytes(pr.M, p.sg2, pr.D);
+    p.o_bytes = slice_bytes(pr.M, p.so2, pr.D);
   }
   if (pr.N > 0) {
     p.sdk0 = kst[0]; p.sdk1 = kst[1]; p.sdk2 = kst[2];
@@ -213,7 +213,6 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   p.causal_off = pr.N - pr.M;
   p.nkb = (int)w.nkb;
   p.nrb = (int)(w.mpad / fas::kBwdBlock);
-  p.nprep = (int)nprep;
   p.wgs = (int)w.wgs;
   p.chunk = (int)w.chunk;
   p.head_tiles = w.head_tiles;

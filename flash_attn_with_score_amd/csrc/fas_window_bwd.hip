@@ -8,8 +8,7 @@ template <class E, int D>
 static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
   const int64_t bh = (int64_t)p.B * p.H, bhk = (int64_t)p.B * p.Hk;
   if (p.M > 0)
-    hipLaunchKernelGGL((bwd_prep_kernel<E, D>), dim3((unsigned)(bh * p.nprep)), dim3(256), 0, s,
-                       p);
+    hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)(bh * p.nrb)), dim3(256), 0, s, p);
   if (p.N > 0) {
     if constexpr (D == 128)
       hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)p.wgs), dim3(512), 0, s, p);
@@ -22,8 +21,6 @@ static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
                          0, s, p);
     }
   }
-  if (p.M > 0)
-    hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)(bh * p.nrb)), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
