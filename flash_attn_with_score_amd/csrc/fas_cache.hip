@@ -4,14 +4,19 @@
 
 namespace fas {
 
-template <class E, int D, int BITS>
-static hipError_t rows_t(const CacheParams& p, bool append, hipStream_t s) {
+template <class E, int D, int BITS, int R>
+static hipError_t rows_r(const CacheParams& p, bool append, hipStream_t s) {
   const dim3 grid((unsigned)(2 * (int64_t)p.B * p.H * p.chunks)), block(256);
   if (append)
-    hipLaunchKernelGGL((cache_append_kernel<E, D, BITS>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((cache_append_kernel<E, D, BITS, R>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((cache_read_kernel<E, D, BITS>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((cache_read_kernel<E, D, BITS, R>), grid, block, 0, s, p);
   return hipGetLastError();
+}
+
+template <class E, int D, int BITS>
+static hipError_t rows_t(const CacheParams& p, bool append, hipStream_t s) {
+  return p.rows == 1 ? rows_r<E, D, BITS, 1>(p, append, s) : rows_r<E, D, BITS, 4>(p, append, s);
 }
 
 template <class E, int D>

@@ -94,9 +94,11 @@ int move_rows(const char* fn, bool append, const fas_kv_cache* c, const void* k,
   if (kst == nullptr || vst == nullptr) return fail(FAS_ERR_INVALID, fn, "k or v strides are NULL");
   if ((rc = check_tensor(fn, "k", k, kst, tokens, c->head_dim))) return rc;
   if ((rc = check_tensor(fn, "v", v, vst, tokens, c->head_dim))) return rc;
-  const int64_t rows = 256 / (c->head_dim / 8);
-  const int64_t chunks = (tokens + rows - 1) / rows;
-  if (2 * c->batch * c->heads * chunks > INT_MAX)
+  // Four rows a thread where that still fills the chip four times over.
+  const int64_t beside = 256 / (c->head_dim / 8), heads = 2 * c->batch * c->heads;
+  const int64_t per = heads * ((tokens + 4 * beside - 1) / (4 * beside)) >= 4 * fas::kCus ? 4 : 1;
+  const int64_t chunks = (tokens + per * beside - 1) / (per * beside);
+  if (heads * chunks > INT_MAX)
     return fail(FAS_ERR_UNSUPPORTED, fn, "more rows than one launch takes");
   fas::CacheParams p{};
   auto side = [](fas::CacheSide& s, const void* rows, const int64_t* st, void* codes,
@@ -117,6 +119,7 @@ int move_rows(const char* fn, bool append, const fas_kv_cache* c, const void* k,
   p.H = (int)c->heads;
   p.M = (int)tokens;
   p.capacity = (int)c->capacity;
+  p.rows = (int)per;
   p.chunks = (int)chunks;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int d = (int)c->head_dim;

@@ -315,6 +315,7 @@ struct CacheParams {
   const int32_t* counts;   // append: (B,) rows written per sequence, or null: M
   int start_all;
   int B, H, M, capacity;
+  int rows;                // rows a thread takes: 1 or 4
   int chunks;              // workgroups per tensor, batch entry and head
 };
 
