@@ -137,9 +137,17 @@ struct CacheSource {
   const int64_t skc, sks, svc, svs;
   uint32_t kw[WPT], vw[WPT], ksb = 0, vsb = 0;
 
+  // The row of the j-th group of threads: neighbours take rows whose chunks the
+  // swizzle puts on different banks (in order, four of the threads that write
+  // at once hit each bank at D = 128: B2 H32/8 M512 N8000 4 bits 233 us, so 210;
+  // two at D = 64, where another order measured the same).
+  static __device__ __forceinline__ int row_of(int j) {
+    return D == 128 ? (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3) : j;
+  }
   __device__ __forceinline__ CacheSource(const RowsParams& p, const RowsPlan& plan_, int b, int hk,
                                          Lds& lds_)
-      : lds(lds_), plan(plan_), row((int)threadIdx.x * UPT / UPR), unit((int)threadIdx.x * UPT % UPR),
+      : lds(lds_), plan(plan_), row(row_of((int)threadIdx.x * UPT / UPR)),
+        unit((int)threadIdx.x * UPT % UPR),
         stager(D >= 32 || (int)threadIdx.x < kRowsKeys * UPR),
         kc(p.k + b * p.sk0 + hk * p.sk1 + unit * BITS),
         ks(p.ks + b * p.sks0 + hk * p.sks1 + unit / 4),

@@ -326,6 +326,8 @@ namespace fas {
 // Most workgroups that share a row's keys (merge_kernel holds one part a
 // thread).
 constexpr int kRowsMaxSplits = 256;
+// Most parts of a row that merge_few_kernel adds up.
+constexpr int kMergeFew = 8;
 // Virtual rows of few_kernel and of a rows_kernel block; their key tiles.
 constexpr int kFewRows = 32, kRowsBlock = 128;
 constexpr int kFewKeys = 32, kRowsKeys = 64;

@@ -25,7 +25,8 @@
 //                 source's business (dense rows by LDS DMA, codes through
 //                 registers); the next tile is under way while the current
 //                 one is used.
-//   merge_kernel  adds up the parts of rows whose keys were dealt to several
+//   merge_few_kernel, merge_kernel
+//                 add up the parts of rows whose keys were dealt to several
 //                 workgroups.
 //
 // Tiles are dealt by the length the device sees, not by the one the host
@@ -728,10 +729,77 @@ void rows_kernel(const RowsParams p) {
 
 // ---------------------------------------------------------------- merge
 
+// The plan of virtual row v, as the kernel that wrote its parts had it.
+template <int BM, int BN>
+__device__ __forceinline__ RowsPlan merge_plan(const RowsParams& p, int b, int v) {
+  RowsPlan c = rows_plan<BM, BN>(p, b, v / BM);
+  if (BM == kFewRows && p.balance) {
+    c.per = *p.part_per;
+    c.used = max(1, (c.tiles + c.per - 1) / c.per);
+  }
+  return c;
+}
+// O (four channels from d0 on) and L of virtual row v, from the parts' sum acc
+// and l relative to the base-2 offset mx.
+template <class E>
+__device__ __forceinline__ void merge_store(const RowsParams& p, const RowsPlan& c, int b, int hk,
+                                            int v, int d0, f32x4 acc, float mx, float l) {
+  const int i = v / p.G, h = hk * p.G + (v - i * p.G);
+  const bool live = i < c.cnt;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.o + b * p.so0 + h * p.so1 + (int64_t)i * p.so2 + d0) =
+      live ? u32x2{E::pack(acc[0] * inv, acc[1] * inv), E::pack(acc[2] * inv, acc[3] * inv)}
+           : u32x2{0u, 0u};
+  if (d0 == 0 && p.lse != nullptr)
+    p.lse[b * p.sl0 + h * p.sl1 + (int64_t)i * p.sl2] =
+        !live || l == 0.f ? neg_inf() : (mx + log2f_fast(l)) * 0.69314718055994531f;
+}
+
 // Row v of KV head bhk: offset M = max of the parts' offsets, weights
-// 2^(m - M), L = sum w l, O = sum w O / L.  One workgroup a row: thread s holds
-// part s's weight, then 1024 / D threads share the parts of each group of four
-// channels.
+// 2^(m - M), L = sum w l, O = sum w O / L.  (A part without an offset has l = 0,
+// or NaN where its scores were.)
+//
+// At most kMergeFew parts a row: D / 4 threads a row, four channels each, all
+// parts' loads under way together.  (A workgroup a row, as below, took 53 us for
+// the 32768 rows in two parts of B2 H32 M512.)
+template <class E, int D, int BM, int BN>
+__global__ __launch_bounds__(256) void merge_few_kernel(const RowsParams p) {
+  constexpr int CH = D / 4, RPB = 256 / CH;
+  const int rows = p.G * p.M, blocks = (rows + RPB - 1) / RPB;
+  const int bhk = (int)(blockIdx.x / (uint32_t)blocks);
+  const int v = (int)(blockIdx.x - (uint32_t)bhk * (uint32_t)blocks) * RPB + (int)threadIdx.x / CH;
+  if (v >= rows) return;
+  const int b = bhk / p.Hk, hk = bhk - b * p.Hk, d0 = 4 * ((int)threadIdx.x % CH);
+  const RowsPlan plan = merge_plan<BM, BN>(p, b, v);
+  if (plan.used == 1) return;
+  const int64_t row0 = (int64_t)bhk * p.nsplit * p.Rpad + v;
+  f32x2 ml[kMergeFew];
+  f32x4 x[kMergeFew];
+  float mx = neg_inf();
+#pragma unroll
+  for (int s = 0; s < kMergeFew; ++s) {
+    const bool has = s < plan.used;
+    const int64_t row = row0 + (int64_t)(has ? s : 0) * p.Rpad;
+    ml[s] = *reinterpret_cast<const f32x2*>(p.part_ml + 2 * row);
+    x[s] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
+    if (!has) ml[s] = f32x2{neg_inf(), 0.f};
+    mx = fmaxf(mx, ml[s].x);
+  }
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll
+  for (int s = 0; s < kMergeFew; ++s) {
+    if (s >= plan.used) continue;
+    const float w = ml[s].x == neg_inf() ? 0.f : exp2f_fast(ml[s].x - mx);
+    l += ml[s].x == neg_inf() ? ml[s].y : w * ml[s].y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[s][e], acc[e]);
+  }
+  merge_store<E>(p, plan, b, hk, v, d0, acc, mx, l);
+}
+
+// More parts: one workgroup a row.  Thread s holds part s's weight, then
+// 1024 / D threads share the parts of each group of four channels.
 template <class E, int D, int BM, int BN>
 __global__ __launch_bounds__(256) void merge_kernel(const RowsParams p) {
   constexpr int CH = D / 4, WAYS = 256 / CH;
@@ -742,11 +810,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const RowsParams p) {
   const int rows = p.G * p.M;
   const int bhk = (int)(blockIdx.x / (uint32_t)rows), v = (int)(blockIdx.x - (uint32_t)bhk * (uint32_t)rows);
   const int b = bhk / p.Hk, hk = bhk - b * p.Hk;
-  RowsPlan plan = rows_plan<BM, BN>(p, b, v / BM);
-  if (BM == kFewRows && p.balance) {
-    plan.per = *p.part_per;
-    plan.used = max(1, (plan.tiles + plan.per - 1) / plan.per);
-  }
+  const RowsPlan plan = merge_plan<BM, BN>(p, b, v);
   if (plan.used == 1) return;
   const int64_t row0 = (int64_t)bhk * p.nsplit * p.Rpad + v;
   static_assert(kRowsMaxSplits == 256, "one part a thread");
@@ -760,7 +824,6 @@ __global__ __launch_bounds__(256) void merge_kernel(const RowsParams p) {
   mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float w = ml.x == neg_inf() ? 0.f : exp2f_fast(ml.x - mx);
   wgt[tid] = w;
-  // (A part without an offset has l = 0, or NaN where its scores were.)
   float l = ml.x == neg_inf() ? ml.y : w * ml.y;
 #pragma unroll
   for (int i = 1; i < 64; i <<= 1) l += __shfl_xor(l, i);
@@ -780,15 +843,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const RowsParams p) {
   __syncthreads();
   if (way != 0) return;
   for (int s = 1; s < WAYS; ++s) acc += part[s][ch];
-  const int i = v / p.G, h = hk * p.G + (v - i * p.G);
-  const bool live = i < plan.cnt;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<u32x2*>(p.o + b * p.so0 + h * p.so1 + (int64_t)i * p.so2 + 4 * ch) =
-      live ? u32x2{E::pack(acc[0] * inv, acc[1] * inv), E::pack(acc[2] * inv, acc[3] * inv)}
-           : u32x2{0u, 0u};
-  if (ch == 0 && p.lse != nullptr)
-    p.lse[b * p.sl0 + h * p.sl1 + (int64_t)i * p.sl2] =
-        !live || l == 0.f ? neg_inf() : (mx + log2f_fast(l)) * 0.69314718055994531f;
+  merge_store<E>(p, plan, b, hk, v, 4 * ch, acc, mx, l);
 }
 
 }  // namespace fas

@@ -6,6 +6,20 @@
 
 namespace fas {
 
+template <class E, int D, int BM, int BN>
+hipError_t launch_merge(const RowsParams& p, hipStream_t s) {
+  const int64_t groups = (int64_t)p.B * p.Hk, rows = p.G * p.M;
+  if (p.nsplit <= kMergeFew) {
+    constexpr int RPB = 1024 / D;
+    hipLaunchKernelGGL((merge_few_kernel<E, D, BM, BN>),
+                       dim3((unsigned)(groups * ((rows + RPB - 1) / RPB))), dim3(256), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((merge_kernel<E, D, BM, BN>), dim3((unsigned)(groups * rows)), dim3(256), 0, s,
+                       p);
+  }
+  return hipGetLastError();
+}
+
 template <class E, int D, class FEW, class MANY>
 hipError_t launch_rows(const RowsParams& p, hipStream_t s) {
   const int rows = p.G * p.M;
@@ -16,13 +30,9 @@ hipError_t launch_rows(const RowsParams& p, hipStream_t s) {
     hipLaunchKernelGGL((few_kernel<E, D, 2, FEW>), grid, block, 0, s, p);
   else
     hipLaunchKernelGGL((rows_kernel<E, D, MANY>), grid, block, 0, s, p);
-  if (p.nsplit > 1) {
-    const dim3 merge((unsigned)((int64_t)p.B * p.Hk * rows));
-    if (rows <= kFewRows)
-      hipLaunchKernelGGL((merge_kernel<E, D, kFewRows, kFewKeys>), merge, block, 0, s, p);
-    else
-      hipLaunchKernelGGL((merge_kernel<E, D, kRowsBlock, kRowsKeys>), merge, block, 0, s, p);
-  }
+  if (p.nsplit > 1)
+    return rows <= kFewRows ? launch_merge<E, D, kFewRows, kFewKeys>(p, s)
+                            : launch_merge<E, D, kRowsBlock, kRowsKeys>(p, s);
   return hipGetLastError();
 }
 
