@@ -44,7 +44,13 @@ inline RowsSplit rows_split(int64_t batch, int64_t groups, int64_t rows, int64_t
   if (blocks > 0 && blocks < kRowsSlots)
     w.nsplit = std::max<int64_t>(1, std::min({(kRowsSlots + blocks - 1) / blocks,
                                               tiles / w.min_tiles, (int64_t)kRowsMaxSplits}));
-  if (few && tiles / 4 - tiles / (4 * w.nsplit) <= 6) w.nsplit = 1;
+  if (few) {
+    // Whole steps: the nearest number of them a workgroup.
+    const int64_t steps = std::max<int64_t>(1, (tiles + 2 * w.nsplit) / (4 * w.nsplit));
+    w.nsplit = std::min<int64_t>(std::max<int64_t>(1, (tiles + 4 * steps - 1) / (4 * steps)),
+                                 kRowsMaxSplits);
+    if (blocks >= kRowsSlots || tiles / 4 - steps <= 6) w.nsplit = 1;
+  }
   w.grid = blocks * w.nsplit;
   // Sequences of unknown lengths (rows_balanced): shorter ones leave workgroups
   // to the longer, up to twice the even share each.  Working it out takes
