@@ -264,12 +264,13 @@ __device__ __forceinline__ void window_store(const WindowBwdParams& p, const Win
     }
 }
 
-// dK, dV up to D = 64: four waves, each with both products of its 32 keys; two
-// workgroups a CU cover each other's waits (the split of the work between two
-// waves that window_dkdv_kernel makes costs them more than it gives, their LDS
-// holding one workgroup a CU: B1 H32 S8192 D64 window 1024, backward, 401 / 477 us).
+// dK, dV up to D = 64, and at D = 128 in fp16: four waves, each with both products
+// of its 32 keys.  Up to D = 64 two workgroups a CU cover each other's waits (the
+// split of the work between two waves that window_dkdv_kernel makes costs them
+// more than it gives, their LDS holding one workgroup a CU: B1 H32 S8192 D64
+// window 1024, backward, 401 / 477 us).
 template <class E, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 1 : 2)))
 void window_dkdv_small_kernel(const WindowBwdParams p) {
   constexpr int KS = D / 16;
   constexpr int DB = D >= 32 ? D / 32 : 1;
@@ -748,21 +749,32 @@ void window_dq_kernel(const WindowBwdParams p) {
     qreg[ks] = buf_load16(rq, (uint32_t)((qrow * p.sq2 + 16 * ks + 8 * g) * 2)) ^ p.qneg;
     greg[ks] = buf_load16(rg, (uint32_t)((qrow * p.sg2 + 16 * ks + 8 * g) * 2));
   }
-  // The row's -delta = -sum_d O dO and nl = -L log2(e), the base-2 exponent offset
-  // of its weights (-inf, so that P is 0, for rows that see no key and for the
-  // padding past M), here and for the dK/dV kernel, which runs next.  (A pass of
-  // its own over O and dO took 14 us of 339 at B1 H32/8 S4096 D128.)
+  // nl = -L log2(e), the base-2 exponent offset of the row's weights (-inf, so
+  // that P is 0, for rows that see no key and for the padding past M), and
+  // -delta = -sum_d O dO, here and for the dK/dV kernel, which runs next.  (A pass
+  // of its own over O and dO took 14 us of 339 at B1 H32/8 S4096 D128.)
   float nl = neg_inf(), xl = 0.f;
-  {
+  if (qrow < p.M) {
+    const float L = p.lse[b * p.sl0 + h * p.sl1 + (int64_t)qrow * p.sl2];
+    if (L != neg_inf()) nl = -L * kLog2e;
+  }
+  // O is rounded to the type, from weights that were.  In rows of few keys O is
+  // as large as V and that is most of the gradients' error (dQ's norm: 1.6 to
+  // 1.77 times a mere rounding's over 100 to 512 causal rows, 1.40 to 1.46 with an
+  // exact delta), so a block whose first row sees 128 keys or fewer forms delta =
+  // sum_j P dP instead, in a sweep of its own over its keys: the first block of a
+  // sequence, which has the shortest list, and all blocks of short windows (the
+  // backward of B1 H32/8 S8192 D64: window 129 94 us, window 128 114 us).  At D = 16,
+  // where rounding dS for its product costs dQ the most, up to 256 keys.
+  const int lo = p.causal_off + row0, hi = min(p.N - 1, lo + BM - 1);
+  constexpr int kFew = D == 16 ? 256 : 128;
+  const bool sweep = lo < p.window ? lo < kFew : min(lo + 1 - p.window, p.sinks) + p.window <= kFew;
+  if (!sweep) {
     const __amdgpu_buffer_rsrc_t ro = make_rsrc(p.o + b * p.so0 + h * p.so1, p.o_bytes);
     u32x4 oreg[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       oreg[ks] = buf_load16(ro, (uint32_t)((qrow * p.so2 + 16 * ks + 8 * g) * 2));
-    if (qrow < p.M) {
-      const float L = p.lse[b * p.sl0 + h * p.sl1 + (int64_t)qrow * p.sl2];
-      if (L != neg_inf()) nl = -L * kLog2e;
-    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       float x[8], y[8];
@@ -772,16 +784,11 @@ void window_dq_kernel(const WindowBwdParams p) {
       for (int e = 0; e < 8; ++e) xl = fmaf(x[e], y[e], xl);
     }
     xl = -xor32_add(xl);
-    if (g == 0) {
-      p.nl[(int64_t)bh * p.Mpad + qrow] = nl;
-      p.delta[(int64_t)bh * p.Mpad + qrow] = xl;
-    }
   }
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]), "+v"(greg[ks]));
 
   // The block's keys as a list, as RowsPlan has it: ns sinks, then the window.
-  const int lo = p.causal_off + row0, hi = min(p.N - 1, lo + BM - 1);
   int ns = 0, shift = 0, hide = 0, ntiles = 0;
   if (hi >= 0) {
     const int first = max(0, lo - p.window + 1);
@@ -806,17 +813,15 @@ void window_dq_kernel(const WindowBwdParams p) {
   f32x16 dq[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
+  float sum = 0.f;
   const float qk = p.qk_scale;
   const VtOff vto = vt_offsets<D>(lane);
   const uint32_t rco = row_chunk_offset<D>(perm_row(c), g);
 
-  if (ntiles > 0) {
-    fetch(0, 0);
-    vm_wait_all();
-    __syncthreads();
-  }
-  auto step = [&](int t, auto stage_tag) __attribute__((always_inline)) {
+  // One tile, towards dQ or (`sums`) towards delta.
+  auto step = [&](int t, auto stage_tag, auto sums_tag) __attribute__((always_inline)) {
     constexpr int stage = decltype(stage_tag)::value;
+    constexpr bool sums = decltype(sums_tag)::value;
     const bool more = t + 1 < ntiles;
     if (more) fetch(t + 1, stage ^ 1);
     const uint16_t* kt = klds[stage];
@@ -867,6 +872,11 @@ void window_dq_kernel(const WindowBwdParams p) {
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = pr[r] * dp[r];
+      if constexpr (sums) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += dp[r];
+        return;
+      }
       const u32x4 sb0 = pack_b<E>(dp, 0), sb1 = pack_b<E>(dp, 1);
       __builtin_amdgcn_sched_barrier(0);
       VtOff o = vto;
@@ -898,10 +908,25 @@ void window_dq_kernel(const WindowBwdParams p) {
     if (more) vm_wait_all();
     __syncthreads();
   };
-  for (int t = 0; t < ntiles; t += 2) {
-    step(t, std::integral_constant<int, 0>{});
-    if (t + 1 < ntiles) step(t + 1, std::integral_constant<int, 1>{});
+  auto all = [&](auto sums_tag) __attribute__((always_inline)) {
+    if (ntiles == 0) return;
+    fetch(0, 0);
+    vm_wait_all();
+    __syncthreads();
+    for (int t = 0; t < ntiles; t += 2) {
+      step(t, std::integral_constant<int, 0>{}, sums_tag);
+      if (t + 1 < ntiles) step(t + 1, std::integral_constant<int, 1>{}, sums_tag);
+    }
+  };
+  if (sweep) {  // (xl is 0: the products are dP itself)
+    all(std::true_type{});
+    xl = -xor32_add(sum);
   }
+  if (g == 0) {
+    p.nl[(int64_t)bh * p.Mpad + qrow] = nl;
+    p.delta[(int64_t)bh * p.Mpad + qrow] = xl;
+  }
+  all(std::false_type{});
 
   // Lane (c, g), register r of block db: row qrow, head dim 32db + acc_row(r, g).
   if (qrow >= p.M) return;

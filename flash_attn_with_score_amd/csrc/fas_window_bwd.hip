@@ -2,6 +2,8 @@
 #include "fas_launch.hpp"
 #include "fas_window.hpp"
 
+#include <type_traits>
+
 namespace fas {
 
 template <class E, int D>
@@ -10,7 +12,10 @@ static hipError_t bwd_t(const WindowBwdParams& p, hipStream_t s) {
   if (p.M > 0)
     hipLaunchKernelGGL((window_dq_kernel<E, D>), dim3((unsigned)(bh * p.nrb)), dim3(256), 0, s, p);
   if (p.N > 0) {
-    if constexpr (D == 128)
+    // Two waves for each 32 keys hand P over in fp16, which loses nothing beside
+    // bf16's own rounding of dS, but would be a second rounding of the same size in
+    // fp16 (dK's norm of error 1.74 times a mere rounding's, 1.43 without it).
+    if constexpr (D == 128 && std::is_same_v<E, BF16>)
       hipLaunchKernelGGL((window_dkdv_kernel<E, D>), dim3((unsigned)p.wgs), dim3(512), 0, s, p);
     else
       hipLaunchKernelGGL((window_dkdv_small_kernel<E, D>), dim3((unsigned)p.wgs), dim3(256), 0, s,

@@ -14,7 +14,8 @@ import torch
 from .cache import visible
 
 
-def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None) -> dict:
+def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None,
+              few_keys: bool = False) -> dict:
     """One batch entry: q, do (Hq, M, D), k, v (Hk, N, D).  Returns out, lse and,
     with do, dq, dk, dv, and under name + "_bound" their bounds.
 
@@ -27,10 +28,14 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None) -> d
     dv: the same over M G terms:  half |dv| + (half + 2 w + 2 M G f) sum P |do|.
     dP - delta: D products each, delta from the rounded out:
       u = 2 (D + 2) f sum |do||v| + (D + 2) f sum |do||out| + sum |do| out_bound
-    (u per pair), and dS = P (dP - delta), rounded for its products:
+    (u per pair); with few_keys (no row block's first row sees more than 128 keys)
+    delta is the sum of P dP over the row's N keys instead, and with a = 2 (D + 2) f
+    sum |do||v|:  u = a + sum_j P a + (2 w + 2 N f) sum_j P |dP|;
+    and dS = P (dP - delta), rounded for its products:
       e = P u + |dS| (half + 2 w + 4 f);
-    for dk P may pass between waves in fp16 (half a step: 2^-12 of its value, 2^-25
-    at least):  e + |dS| 2^-12 + |dP - delta| 2^-25 where the pair is visible.
+    for dk of a bf16 call P may pass between waves in fp16 (half a step: 2^-11 of its
+    value, 2^-25 at least):  e + |dS| 2^-11 + |dP - delta| 2^-25 where the pair is
+    visible.
     dq: half |dq| + s sum_j (e + 2 N f |dS|) |k|;  dk alike over rows."""
     Hq, M, D = q.shape
     Hk, N = k.shape[:2]
@@ -60,15 +65,19 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None) -> d
     res["dv"] = fold(P.transpose(1, 2) @ do)
     res["dq"] = (dS @ kx) * scale
     res["dk"] = fold(dS.transpose(1, 2) @ q) * scale
-    u = 2 * (D + 2) * f * (do.abs() @ vx.abs().transpose(1, 2)) \
-        + ((D + 2) * f * (do * out).abs() + do.abs() * res["out_bound"]).sum(-1, keepdim=True)
+    u = 2 * (D + 2) * f * (do.abs() @ vx.abs().transpose(1, 2))
+    if few_keys:
+        u = u + (P * u).sum(-1, keepdim=True) + (2 * w + 2 * N * f) * (P * dP.abs()).sum(-1, keepdim=True)
+    else:
+        u = u + ((D + 2) * f * (do * out).abs() + do.abs() * res["out_bound"]).sum(-1, keepdim=True)
     e = P * u + dS.abs() * (half + 2 * w + 4 * f)
     res["dv_bound"] = half * res["dv"].abs() + tiny + (half + 2 * w + 2 * M * G * f) * (1 + half) \
         * fold(P.transpose(1, 2) @ do.abs())
     res["dq_bound"] = half * res["dq"].abs() + tiny + (1 + half) * abs(scale) \
         * ((e + 2 * N * f * dS.abs()) @ kx.abs())
-    e = e + dS.abs() * 2.0 ** -12 + torch.where(see, 2.0 ** -25, 0.0) \
-        * (dP - (do * out).sum(-1, keepdim=True)).abs()
+    if half == 2.0 ** -8:
+        e = e + dS.abs() * 2.0 ** -11 + torch.where(see, 2.0 ** -25, 0.0) \
+            * (dP - (do * out).sum(-1, keepdim=True)).abs()
     res["dk_bound"] = half * res["dk"].abs() + tiny + (1 + half) * abs(scale) \
         * fold((e + 2 * M * G * f * dS.abs()).transpose(1, 2) @ q.abs())
     return res

@@ -17,7 +17,7 @@ FP16, BF16 = torch.float16, torch.bfloat16
 
 
 def check(gpu, B, Hq, Hk, M, N, D, dtype, window, sinks, grad=True, layout="bhsd", sm_scale=None,
-          seed=0, scale=1.0):
+          seed=0, scale=1.0, few_keys=False):
     print(f"[case] window B{B}H{Hq}K{Hk}M{M}N{N}D{D} {dtype} window={window} sinks={sinks} "
           f"grad={grad} {layout}", flush=True)
     q, k, v = inputs.make_qkv(B, Hq, Hk, M, N, D, dtype=dtype, seed=seed, scale=scale)
@@ -37,7 +37,7 @@ def check(gpu, B, Hq, Hk, M, N, D, dtype, window, sinks, grad=True, layout="bhsd
     torch.cuda.synchronize()
     for b in range(B):
         ref = oracle.reference(q[b], k[b], v[b], min(window, 1 << 40), min(sinks, 1 << 40),
-                               do[b] if grad else None, sm_scale)
+                               do[b] if grad else None, sm_scale, few_keys)
         empty = torch.isinf(ref["lse"])
         assert torch.equal(got["lse"][b].cpu() == -math.inf, empty)
         assert (got["out"][b].cpu()[empty] == 0).all()
@@ -54,6 +54,15 @@ def check(gpu, B, Hq, Hk, M, N, D, dtype, window, sinks, grad=True, layout="bhsd
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 def test_instances(D, dtype, gpu):
     check(gpu, 2, 4, 2, 300, 300, D, dtype, 70, 5, seed=D)
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+@pytest.mark.parametrize("M,N,window,sinks", [(128, 128, 500, 0), (90, 100, 80, 4), (120, 100, 200, 1),
+                                              (500, 500, 100, 28), (300, 410, 64, 64), (333, 333, 1, 0)])
+def test_rows_of_few_keys(M, N, window, sinks, D, gpu):
+    """No block's first row sees more than 128 keys: out's rounding does not reach
+    the gradients."""
+    check(gpu, 1, 4, 2, M, N, D, (FP16, BF16)[D % 128 == 0], window, sinks, seed=M + D, few_keys=True)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 200), (31, 0), (32, 32), (33, 31),
