@@ -39,6 +39,13 @@ def as_kernel_operand(x: torch.Tensor) -> torch.Tensor:
     return x if _rows_aligned(x) else x.contiguous()
 
 
+def as_row_operand(x: torch.Tensor) -> torch.Tensor:
+    """as_kernel_operand of a tensor whose rows may overlap as well (one that is
+    expanded over its tokens): those are copied."""
+    x = as_kernel_operand(x)
+    return x if x.stride(2) >= x.shape[3] else x.clone(memory_format=torch.contiguous_format)
+
+
 @dataclass
 class Problem:
     q: torch.Tensor

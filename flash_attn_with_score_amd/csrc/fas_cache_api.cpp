@@ -71,6 +71,16 @@ int check_cache(const char* fn, const fas_kv_cache* c) {
   return check_cache_array(fn, "v_scales", c->v_scales, c->v_scales_stride, scales);
 }
 
+// Rows that are written: no two sequences, heads or sides in one place.
+int check_distinct(const char* fn, const fas_kv_cache* c) {
+  for (const int64_t* st : {c->k_codes_stride, c->v_codes_stride, c->k_scales_stride, c->v_scales_stride})
+    if ((c->batch > 1 && st[0] == 0) || (c->heads > 1 && st[1] == 0))
+      return fail(FAS_ERR_INVALID, fn, "the cache's rows repeat (stride 0): it cannot be written");
+  if (c->k_codes == c->v_codes || c->k_scales == c->v_scales)
+    return fail(FAS_ERR_INVALID, fn, "keys and values share an array: it cannot be written");
+  return FAS_OK;
+}
+
 int check_per_sequence(const char* fn, const char* name, const int32_t* ptr) {
   if (reinterpret_cast<uintptr_t>(ptr) % 4)
     return fail(FAS_ERR_INVALID, fn, "%s must be aligned to 4 bytes", name);
@@ -88,12 +98,13 @@ int move_rows(const char* fn, bool append, const fas_kv_cache* c, const void* k,
   if ((rc = check_per_sequence(fn, "start", start))) return rc;
   if ((rc = check_per_sequence(fn, "counts", counts))) return rc;
   if (start == nullptr && (start_all < 0 || start_all > c->capacity - tokens))
-    return fail(FAS_ERR_INVALID, fn, "rows [%lld, %lld) lie outside the cache of %lld",
-                (long long)start_all, (long long)(start_all + tokens), (long long)c->capacity);
+    return fail(FAS_ERR_INVALID, fn, "%lld rows from %lld lie outside the cache of %lld",
+                (long long)tokens, (long long)start_all, (long long)c->capacity);
   if (c->batch == 0 || tokens == 0) return FAS_OK;
   if (kst == nullptr || vst == nullptr) return fail(FAS_ERR_INVALID, fn, "k or v strides are NULL");
   if ((rc = check_tensor(fn, "k", k, kst, tokens, c->head_dim))) return rc;
   if ((rc = check_tensor(fn, "v", v, vst, tokens, c->head_dim))) return rc;
+  if (append && c->capacity > 0 && (rc = check_distinct(fn, c))) return rc;
   // Four rows a thread where that still fills the chip four times over.
   const int64_t beside = 256 / (c->head_dim / 8), heads = 2 * c->batch * c->heads;
   const int64_t per = heads * ((tokens + 4 * beside - 1) / (4 * beside)) >= 4 * fas::kCus ? 4 : 1;

@@ -21,6 +21,7 @@ them is differentiable.
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass, field
 
 import torch
@@ -38,7 +39,9 @@ class KVCache:
     bits / 8) and scales (batch, heads_k, capacity, max(1, head_dim / 32)) of the
     keys and of the values, the type of the values and the bits of a code.  An
     array's rows must be contiguous and aligned to their size (up to 16 bytes);
-    its other strides are free.  include/fas.h says what the bytes mean."""
+    its other strides are free (only a cache that is not appended to may repeat
+    rows, a prompt that its sequences share, say).  The arrays' memory has to stay
+    where it is.  include/fas.h says what the bytes mean."""
 
     k_codes: torch.Tensor
     k_scales: torch.Tensor
@@ -70,6 +73,9 @@ class KVCache:
         assert all(t.stride(3) == 1 or t.shape[3] == 1 for t in arrays), "rows must be contiguous"
         object.__setattr__(self, "head_dim", D)
         object.__setattr__(self, "_record", _native.pack_kv_cache(*arrays, self.dtype, self.bits, D))
+
+    def __reduce__(self):  # a copy has arrays, and so addresses, of its own
+        return (KVCache, (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.dtype, self.bits))
 
     @property
     def batch(self) -> int:
@@ -104,7 +110,7 @@ def kv_cache(batch: int, heads_k: int, capacity: int, head_dim: int, bits: int =
 def _per_sequence(name: str, x, cache: KVCache):
     """(tensor or None, int) of a per-sequence number."""
     if not isinstance(x, torch.Tensor):
-        return None, int(x)
+        return None, operator.index(x)
     assert x.dtype == torch.int32 and tuple(x.shape) == (cache.batch,), \
         f"{name} must be an int or an int32 tensor of {cache.batch} elements"
     if not x.is_cuda:
@@ -152,7 +158,7 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start, cou
     counts_t = _counts(counts, cache)
     if start_t is None:
         _span("kv_cache_append", start_all, M, cache)
-    k, v = _common.as_kernel_operand(k), _common.as_kernel_operand(v)
+    k, v = _common.as_row_operand(k), _common.as_row_operand(v)
     _common.call("fas_kv_cache_append", cache.k_codes, cache._record, k.data_ptr(),
                  _native.pack_strides(k), v.data_ptr(), _native.pack_strides(v), M, _ptr(start_t),
                  start_all, _ptr(counts_t))
@@ -213,7 +219,7 @@ def attention_kv_cache(q: torch.Tensor, cache: KVCache, lengths, counts=None,
     if lengths_t is None and not 0 <= lengths_all <= cache.capacity:
         raise ValueError(f"flash_attn_with_score_amd: length {lengths_all} lies outside "
                          f"[0, {cache.capacity}]")
-    q = _common.as_kernel_operand(q)
+    q = _common.as_row_operand(q)
     out = _common.new_output(q)
     lse = torch.empty((B, H, M), dtype=torch.float32, device=q.device) if return_log_normalizer \
         else None

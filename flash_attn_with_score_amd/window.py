@@ -58,7 +58,7 @@ def _check_capture(ctx, device) -> None:
 
 
 def _forward(q, k, v, window, sinks, sm_scale, want_lse):
-    p = _common.finish_problem(q, k, v, sm_scale)
+    p = _common.finish_problem(*(_common.as_row_operand(x) for x in (q, k, v)), sm_scale)
     o = _common.new_output(p.q)
     L = torch.empty((p.B, p.H, p.M), device=q.device, dtype=torch.float32) if want_lse else None
     args = _native.pack_args(p.q, p.k, p.v, o, True, p.sm_scale)
@@ -84,9 +84,12 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, *ignored):
+        if torch.is_grad_enabled():
+            raise RuntimeError("flash_attn_with_score_amd: attention_window is differentiable once "
+                               "(create_graph=True)")
         q, k, v, o, L = ctx.saved_tensors
         _check_capture(ctx, q.device)
-        do = _common.as_kernel_operand(do)
+        do = _common.as_row_operand(do)
         dq, dk, dv = _common.new_output(q), _common.new_output(k), _common.new_output(v)
         args = _native.pack_args(q, k, v, o, True, ctx.sm_scale)
         ws_ptr, ws_bytes, ws = _workspace(args, ctx.window, ctx.sinks, 1, q.device)
@@ -105,7 +108,7 @@ def attention_window(q, k, v, window: int, sinks: int = 0, sm_scale: float | Non
 
     Returns out like q, or (out, log_normalizer (B, Hq, M) fp32, which is not
     differentiable).  Rows that see no key (M > N) are 0, their normalizer -inf.
-    Differentiable in q, k and v; like attention(), it takes finite inputs: a
+    Differentiable once in q, k and v; like attention(), it takes finite inputs: a
     hidden key has weight 0, and 0 times an infinity or NaN in it is NaN."""
     _check_inputs(q, k, v)
     _common.check_device_inputs(q, k, v, 0.0)

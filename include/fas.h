@@ -343,7 +343,9 @@ typedef struct fas_kv_cache {
  * power of two s (at least 2^-126) with amax <= C s, C = 6 or 448, but no
  * larger than keeps C s finite in the value type (2^13 and 2^7 for fp16, 2^125
  * and 2^119 for bf16); values round to the nearest code, ties to even, those
- * past C s to C s.  A block with an infinity or NaN reads as NaN. */
+ * past C s to C s.  A block with an infinity or NaN reads as NaN.  A cache whose
+ * sequences or heads repeat (stride 0), or whose keys and values are one array,
+ * can be read and attended over, not written. */
 int fas_kv_cache_append(const fas_kv_cache* cache, const void* k, const int64_t k_stride[4],
                         const void* v, const int64_t v_stride[4], int64_t tokens,
                         const int32_t* start, int64_t start_all, const int32_t* counts,

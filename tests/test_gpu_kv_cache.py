@@ -5,6 +5,7 @@ the bounds that oracle/cache.py: attend_bounds derives.
 """
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
@@ -414,5 +415,42 @@ def test_refusals(gpu):
     with pytest.raises(AssertionError):
         KVCache(c, s, c, s, dtype=BF16, bits=5)
     wide = torch.zeros((2, 2, 8, 24), dtype=torch.uint8, device=gpu)[..., 4:20]
+    with pytest.raises(TypeError):
+        attention_kv_cache(q, cache, 2.5)
+    shared = KVCache(*(t[:1].expand(2, -1, -1, -1) for t in (c, s, cache.v_codes, cache.v_scales)),
+                     dtype=BF16, bits=4)
+    with pytest.raises(RuntimeError, match="repeat"):
+        kv_cache_append(shared, x, x, 0)
+    with pytest.raises(RuntimeError, match="share"):
+        kv_cache_append(KVCache(c, s, c, s, dtype=BF16, bits=4), x, x, 0)
     with pytest.raises(RuntimeError, match="aligned"):
         kv_cache_append(KVCache(wide, s, c, s, dtype=BF16, bits=4), x, x, 0)
+
+
+def test_copies_and_shared_prompts(gpu):
+    """A copied or pickled cache has arrays of its own; sequences may share a
+    cache that is not appended to; rows expanded over tokens and heads are taken."""
+    print("[case] copies", flush=True)
+    B, Hk, M, D = 3, 2, 50, 64
+    cache = kv_cache(B, Hk, 64, D, device=gpu)
+    row = torch.randn(D, generator=torch.Generator("cpu").manual_seed(1)).to(BF16).to(gpu)
+    x = row.expand(B, Hk, M, D)
+    kv_cache_append(cache, x, x, 0)
+    twin = copy.deepcopy(cache)
+    kv_cache_append(twin, torch.zeros_like(x), torch.zeros_like(x), 0)
+    for y in kv_cache_read(cache, 0, M):
+        want = oracle.decode(*oracle.quantise(row.cpu()[None], 4), 4)[0]
+        assert torch.equal(y.cpu().double(), want.expand(B, Hk, M, D))
+    assert all((y == 0).all() for y in kv_cache_read(twin, 0, M))
+    y = torch.randn(B, Hk, M, D, generator=torch.Generator("cpu").manual_seed(2)).to(BF16).to(gpu)
+    kv_cache_append(cache, y, y.flip(2), 0)
+    shared = KVCache(*(t[1:2].expand(B, -1, -1, -1) for t in
+                       (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)), dtype=BF16, bits=4)
+    q = torch.randn(B, 4, 2, D, generator=torch.Generator("cpu").manual_seed(3)).to(BF16).to(gpu)
+    got = attention_kv_cache(q, shared, M)
+    for b in range(B):
+        one = KVCache(*(t[1:2] for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)),
+                      dtype=BF16, bits=4)
+        assert torch.equal(got[b:b + 1], attention_kv_cache(q[b:b + 1].contiguous(), one, M))
+    qx = q[:, :, :1].expand(B, 4, 5, D)
+    assert torch.equal(attention_kv_cache(qx, cache, M), attention_kv_cache(qx.contiguous(), cache, M))

@@ -134,6 +134,23 @@ def test_unaligned_and_broadcast_inputs(gpu):
     assert ((gk[0, 0].cpu().double() - want).abs() <= bound).all()
 
 
+def test_gradients_of_token_sums(gpu):
+    """A dO that is expanded over the tokens, as a sum over them hands it on."""
+    B, H, M, D = 1, 4, 90, 64
+    q, k, v = (x.to(gpu).requires_grad_(True) for x in inputs.make_qkv(B, H, H, M, M, D, dtype=FP16, seed=4))
+    w = torch.randn(B, H, D, generator=torch.Generator("cpu").manual_seed(5)).to(FP16).to(gpu)
+    out = attention_window(q, k, v, 40, 1)
+    got = torch.autograd.grad(out, (q, k, v), w[:, :, None].expand(B, H, M, D), retain_graph=True)
+    want = torch.autograd.grad(out, (q, k, v), w[:, :, None].expand(B, H, M, D).contiguous())
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_second_derivatives_are_refused(gpu):
+    q, k, v = (x.to(gpu).requires_grad_(True) for x in inputs.make_qkv(1, 2, 2, 40, 40, 32, dtype=FP16, seed=4))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(attention_window(q, k, v, 16).sum(), q, create_graph=True)
+
+
 def test_captured_training_step(gpu):
     """Forward and backward in one graph; every replay equals the eager step."""
     B, H, Hk, M, D = 1, 4, 2, 260, 64

@@ -45,6 +45,7 @@ def attn_args(B=1, Hq=4, Hk=2, M=300, N=300, D=64, causal=1, dtype=1):
 
 
 def cache_args(B=2, H=2, N=100, D=64, bits=4, dtype=1):
+    """(Keys and values at one address: an append of it is refused.)"""
     c = _native.KVCacheArgs()
     c.dtype, c.bits, c.batch, c.heads, c.capacity, c.head_dim = dtype, bits, B, H, N, D
     code, scale = D * bits // 8, max(1, D // 32)
@@ -219,6 +220,23 @@ def test_cache_refuses_rows(lib):
     st = _native._I64x4(0, 0, 64, 1)
     refused(lib, untyped(lib, "fas_kv_cache_read", None, P, st, P, st, n5, None, zero, None),
             _native.FAS_ERR_INVALID, "cache is NULL")
+
+
+def test_append_refuses_rows_in_one_place(lib):
+    for n in ("k_codes", "v_scales"):
+        for at in (0, 1):
+            c = cache_args()
+            row = 32 if "codes" in n else 2
+            st = [200 * row, 100 * row, row]
+            st[at] = 0
+            setattr(c, n + "_stride", _native._I64x3(*st))
+            for part in ("codes", "scales"):  # distinct otherwise
+                setattr(c, "v_" + part, PTR + (1 << 30))
+            refused(lib, move(lib, c), _native.FAS_ERR_INVALID, "repeat")
+    refused(lib, move(lib, cache_args()), _native.FAS_ERR_INVALID, "share")
+    c = cache_args()
+    c.v_codes = PTR + (1 << 30)
+    refused(lib, move(lib, c), _native.FAS_ERR_INVALID, "share")
 
 
 def test_attention_refuses_queries(lib):
