@@ -47,8 +47,8 @@ hipError_t launch_cache_append(const CacheParams& p, int dtype, int d, int bits,
 hipError_t launch_cache_read(const CacheParams& p, int dtype, int d, int bits, hipStream_t s);
 hipError_t launch_cache_attn(const RowsParams& p, int dtype, int d, int bits, hipStream_t s);
 
-// Windowed attention over dense keys (fas_window.hpp) and its backward: prep,
-// dK/dV (+ reduction), dQ.
+// Windowed attention over dense keys (fas_window.hpp) and its backward: dQ, dK/dV
+// (+ the sum of parts).
 hipError_t launch_window_fwd(const RowsParams& p, int dtype, int d, hipStream_t s);
 hipError_t launch_window_bwd(const WindowBwdParams& p, int dtype, int d, hipStream_t s);
 

@@ -455,15 +455,14 @@ void window_dkdv_small_kernel(const WindowBwdParams p) {
   } while (run.next(p));
 }
 
-// dK, dV: eight waves, two for each 32 keys of the block: one turns S into P and
+// dK, dV at D = 128 in bf16: eight waves, two for each 32 keys: one turns S into P and
 // accumulates dV, the other turns dP into dS and accumulates dK, a tile later,
 // with the P that the first left in LDS.  Each does half the products and holds
 // half the accumulators, so two waves a SIMD fit (one that did both took 350
 // registers), and one's exponentials and waits run beside the other's products
-// (B1 H32/8 S4096 D128 window 1024: 204 us, with
-// one wave a SIMD for both 212).  P passes in fp16 whatever the input
-// type: within 2^-12 of its value, and 2^-25 below fp16's normal range, both
-// beside the rounding of dS itself.
+// (the backward of B1 H32/8 S8192 D128 window 4096: 1533 us, with one wave for
+// both 1647).  P passes in fp16: within 2^-11 of its value, and 2^-25 below fp16's
+// normal range, an eighth of what rounding dS to bf16 takes.
 template <int D>
 struct WindowDkdvLds {
   uint16_t q[3][64 * D], g[3][64 * D];  // Q and dO
