@@ -36,6 +36,9 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None,
     for dk of a bf16 call P may pass between waves in fp16 (half a step: 2^-11 of its
     value, 2^-25 at least):  e + |dS| 2^-11 + |dP - delta| 2^-25 where the pair is
     visible.
+    A weight below 2^-126, fp32's least normal number, counts as 0 (exp2 returns no
+    subnormals): that leaves 2^-126 |v| out of out, 2^-126 |do| out of dv and 2^-126
+    |dP - delta| out of dS.
     dq: half |dq| + s sum_j (e + 2 N f |dS|) |k|;  dk alike over rows."""
     Hq, M, D = q.shape
     Hk, N = k.shape[:2]
@@ -54,7 +57,8 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None,
     P = torch.exp(s - torch.where(torch.isinf(lse), 0.0, lse)[..., None])
     out = P @ vx
     res = {"out": out, "lse": lse}
-    res["out_bound"] = half * out.abs() + (half + 2 * w + 2 * N * f) * (1 + half) * (P @ vx.abs()) + tiny
+    least = 2.0 ** -126 * see.double().expand(Hq, M, N)
+    res["out_bound"] = half * out.abs() + (half + 2 * w + 2 * N * f) * (1 + half) * (P @ vx.abs()) + least @ vx.abs() + tiny
     res["lse_bound"] = w + N * f + 4 * f * (1 + torch.where(torch.isinf(lse), 0.0, lse.abs()))
     if do is None:
         return res
@@ -70,14 +74,14 @@ def reference(q, k, v, window: int, sinks: int = 0, do=None, sm_scale=None,
         u = u + (P * u).sum(-1, keepdim=True) + (2 * w + 2 * N * f) * (P * dP.abs()).sum(-1, keepdim=True)
     else:
         u = u + ((D + 2) * f * (do * out).abs() + do.abs() * res["out_bound"]).sum(-1, keepdim=True)
-    e = P * u + dS.abs() * (half + 2 * w + 4 * f)
+    gap = (dP - (do * out).sum(-1, keepdim=True)).abs()
+    e = P * u + dS.abs() * (half + 2 * w + 4 * f) + least * gap
     res["dv_bound"] = half * res["dv"].abs() + tiny + (half + 2 * w + 2 * M * G * f) * (1 + half) \
-        * fold(P.transpose(1, 2) @ do.abs())
+        * fold(P.transpose(1, 2) @ do.abs()) + fold(least.transpose(1, 2) @ do.abs())
     res["dq_bound"] = half * res["dq"].abs() + tiny + (1 + half) * abs(scale) \
         * ((e + 2 * N * f * dS.abs()) @ kx.abs())
     if half == 2.0 ** -8:
-        e = e + dS.abs() * 2.0 ** -11 + torch.where(see, 2.0 ** -25, 0.0) \
-            * (dP - (do * out).sum(-1, keepdim=True)).abs()
+        e = e + dS.abs() * 2.0 ** -11 + torch.where(see, 2.0 ** -25, 0.0) * gap
     res["dk_bound"] = half * res["dk"].abs() + tiny + (1 + half) * abs(scale) \
         * fold((e + 2 * M * G * f * dS.abs()).transpose(1, 2) @ q.abs())
     return res

@@ -231,6 +231,48 @@ def test_attend_long(M, G, gpu):
     check_attend(gpu, G, 1, M, 9000, 128, 8, FP16, [8999, 3000], window=2500, sinks=70, seed=6)
 
 
+@pytest.mark.parametrize("B", [2, 64, 65, 70])
+def test_attend_many_sequences(B, gpu):
+    """Batches that are and are not dealt by length, most of them short."""
+    lengths = [(7 * b * b) % 400 for b in range(B)]
+    lengths[1], lengths[-1] = 12000, 5000
+    check_attend(gpu, 2, 1, 1, 12000, 32, 4, BF16, lengths, seed=12)
+    check_attend(gpu, 3, 1, 2, 12000, 16, 8, FP16, lengths, window=7000, sinks=1, seed=13)
+
+
+def test_attend_streams_and_graphs(gpu):
+    """Calls on two streams at once, and two graphs that share a memory pool,
+    replayed in turn: no call sees another's workspace."""
+    B, Hq, Hk, cap, D = 2, 8, 2, 9000, 64
+    calls = []
+    for seed, lens in ((1, [9000, 3]), (2, [4000, 8000])):
+        cache, _ = filled(gpu, B, Hk, cap, D, 4, BF16, 40 + seed)
+        q = rows((B, Hq, 1, D), BF16, 50 + seed).to(gpu)
+        calls.append((q, cache, torch.tensor(lens, dtype=torch.int32, device=gpu)))
+    want = [attention_kv_cache(*c) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for _ in range(4):
+        for c, s in zip(calls, streams):
+            with torch.cuda.stream(s):
+                got.append(attention_kv_cache(*c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(attention_kv_cache(*c))
+        graphs.append(g)
+    for _ in range(3):
+        for g, x, y in zip(graphs, outs, want):
+            x.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(x, y)
+
+
 def test_attend_scales_and_layouts(gpu):
     check_attend(gpu, 4, 2, 3, 200, 64, 4, FP16, [200, 77], sm_scale=-0.3, seed=7)
     check_attend(gpu, 4, 2, 50, 200, 64, 4, BF16, [200, 77], sm_scale=0.0, layout="bshd", seed=8)

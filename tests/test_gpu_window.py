@@ -101,6 +101,23 @@ def test_long_windows_split(gpu):
     check(gpu, 1, 4, 4, 1500, 1700, 128, FP16, 129, 1, seed=10)
 
 
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_key_blocks_dealt_to_several_workgroups(D, dtype, gpu):
+    """Sinks that all later rows see beside short windows: parts of key blocks, runs
+    over several blocks and heads, blocks that no row sees."""
+    check(gpu, 2, 4, 2, 1300, 1300, D, dtype, 40, 130, seed=21)
+    check(gpu, 1, 2, 2, 900, 2100, D, dtype, 129, 33, seed=22)
+    check(gpu, 1, 6, 1, 700, 500, D, dtype, 33, 1, seed=23)
+
+
+@pytest.mark.parametrize("D,dtype", [(32, FP16), (64, BF16), (128, FP16), (128, BF16)])
+def test_scores_of_hundreds(D, dtype, gpu):
+    """Rows whose maximum rises from tile to tile, and weights that vanish."""
+    check(gpu, 1, 4, 2, 300, 300, D, dtype, 150, 4, seed=24, scale=6.0)
+    check(gpu, 1, 4, 2, 2, 1100, D, dtype, 900, 4, seed=25, scale=6.0)
+
+
 def test_window_past_the_keys_is_causal_attention(gpu):
     q, k, v = (t.to(gpu) for t in inputs.make_qkv(2, 4, 2, 333, 333, 128, dtype=FP16, seed=11))
     out, lse = attention_window(q, k, v, 333, return_log_normalizer=True)
