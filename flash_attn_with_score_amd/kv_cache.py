@@ -50,6 +50,10 @@ class KVCache:
     dtype: torch.dtype
     bits: int
     head_dim: int = field(init=False)
+    batch: int = field(init=False)
+    heads_k: int = field(init=False)
+    capacity: int = field(init=False)
+    device: torch.device = field(init=False)
     _record: bytes = field(init=False, repr=False)
 
     def __post_init__(self):
@@ -71,27 +75,13 @@ class KVCache:
         assert self.k_scales.shape == self.v_scales.shape == (B, H, N, blocks), \
             f"scales must be {(B, H, N, blocks)}"
         assert all(t.stride(3) == 1 or t.shape[3] == 1 for t in arrays), "rows must be contiguous"
-        object.__setattr__(self, "head_dim", D)
-        object.__setattr__(self, "_record", _native.pack_kv_cache(*arrays, self.dtype, self.bits, D))
+        record = _native.pack_kv_cache(*arrays, self.dtype, self.bits, D)
+        for name, value in (("head_dim", D), ("batch", B), ("heads_k", H), ("capacity", N),
+                            ("device", self.k_codes.device), ("_record", record)):
+            object.__setattr__(self, name, value)
 
     def __reduce__(self):  # a copy has arrays, and so addresses, of its own
         return (KVCache, (self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.dtype, self.bits))
-
-    @property
-    def batch(self) -> int:
-        return self.k_codes.shape[0]
-
-    @property
-    def heads_k(self) -> int:
-        return self.k_codes.shape[1]
-
-    @property
-    def capacity(self) -> int:
-        return self.k_codes.shape[2]
-
-    @property
-    def device(self) -> torch.device:
-        return self.k_codes.device
 
 
 def kv_cache(batch: int, heads_k: int, capacity: int, head_dim: int, bits: int = 4,
@@ -111,7 +101,7 @@ def _per_sequence(name: str, x, cache: KVCache):
     """(tensor or None, int) of a per-sequence number."""
     if not isinstance(x, torch.Tensor):
         return None, operator.index(x)
-    assert x.dtype == torch.int32 and tuple(x.shape) == (cache.batch,), \
+    assert x.dtype == torch.int32 and x.shape == (cache.batch,), \
         f"{name} must be an int or an int32 tensor of {cache.batch} elements"
     if not x.is_cuda:
         raise RuntimeError(f"flash_attn_with_score_amd: {name} must be a HIP device tensor")
@@ -146,14 +136,16 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, start, cou
     its values (the largest of the type excepted, include/fas.h), and its values
     round to the nearest code, ties to even; a block that holds an infinity or
     NaN reads back as NaN."""
-    want = (cache.batch, cache.heads_k, k.shape[2] if k.dim() == 4 else -1, cache.head_dim)
-    assert tuple(k.shape) == want and tuple(v.shape) == want, \
-        f"k and v must be {want[:2]} x M x {cache.head_dim}, got {tuple(k.shape)}, {tuple(v.shape)}"
+    shape = k.shape
+    assert shape == v.shape and len(shape) == 4 and \
+        (shape[0], shape[1], shape[3]) == (cache.batch, cache.heads_k, cache.head_dim), \
+        f"k and v must be {cache.batch} x {cache.heads_k} x M x {cache.head_dim}, " \
+        f"got {tuple(k.shape)}, {tuple(v.shape)}"
     assert k.dtype == cache.dtype and v.dtype == cache.dtype, f"k and v must be {cache.dtype}"
     if not (k.is_cuda and v.is_cuda):
         raise RuntimeError("flash_attn_with_score_amd: k and v must be HIP device tensors")
     assert k.device == cache.device and v.device == cache.device, "k and v must be on the cache's device"
-    M = k.shape[2]
+    M = shape[2]
     start_t, start_all = _per_sequence("start", start, cache)
     counts_t = _counts(counts, cache)
     if start_t is None:
@@ -178,10 +170,11 @@ def kv_cache_read(cache: KVCache, start=0, length: int | None = None):
     if start_t is None:
         _span("kv_cache_read", start_all, length, cache)
     shape = (cache.batch, cache.heads_k, length, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
-    _common.call("fas_kv_cache_read", cache.k_codes, cache._record, k.data_ptr(),
-                 _native.pack_strides(k), v.data_ptr(), _native.pack_strides(v), length,
-                 _ptr(start_t), start_all)
+    k = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+    v = torch.empty_like(k)
+    strides = _native.pack_strides(k)
+    _common.call("fas_kv_cache_read", cache.k_codes, cache._record, k.data_ptr(), strides,
+                 v.data_ptr(), strides, length, _ptr(start_t), start_all)
     return k, v
 
 
