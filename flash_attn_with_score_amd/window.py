@@ -10,6 +10,9 @@ cache.
 """
 from __future__ import annotations
 
+import math
+import operator
+
 import torch
 
 from . import _common, _native
@@ -58,15 +61,16 @@ def _check_capture(ctx, device) -> None:
 
 
 def _forward(q, k, v, window, sinks, sm_scale, want_lse):
-    p = _common.finish_problem(*(_common.as_row_operand(x) for x in (q, k, v)), sm_scale)
-    o = _common.new_output(p.q)
-    L = torch.empty((p.B, p.H, p.M), device=q.device, dtype=torch.float32) if want_lse else None
-    args = _native.pack_args(p.q, p.k, p.v, o, True, p.sm_scale)
+    """(q, k, v as the kernels take them, out, normalizer or None)."""
+    q, k, v = _common.as_row_operand(q), _common.as_row_operand(k), _common.as_row_operand(v)
+    o = _common.new_output(q)
+    L = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32) if want_lse else None
+    args = _native.pack_args(q, k, v, o, True, sm_scale)
     ws_ptr, ws_bytes, ws = _workspace(args, window, sinks, 0, q.device)
-    _common.call("fas_attention_window", p.q, args, window, sinks,
+    _common.call("fas_attention_window", q, args, window, sinks,
                  0 if L is None else L.data_ptr(), None if L is None else _native.pack_strides(L),
                  ws_ptr, ws_bytes)
-    return p, o, L
+    return q, k, v, o, L
 
 
 class WindowAttention(torch.autograd.Function):
@@ -74,9 +78,9 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, sm_scale, return_log_normalizer):
-        p, o, L = _forward(q, k, v, window, sinks, sm_scale, True)
-        ctx.save_for_backward(p.q, p.k, p.v, o, L)
-        ctx.window, ctx.sinks, ctx.sm_scale = window, sinks, p.sm_scale
+        q, k, v, o, L = _forward(q, k, v, window, sinks, sm_scale, True)
+        ctx.save_for_backward(q, k, v, o, L)
+        ctx.window, ctx.sinks, ctx.sm_scale = window, sinks, sm_scale
         if return_log_normalizer:
             ctx.mark_non_differentiable(L)
             return o, L
@@ -116,9 +120,10 @@ def attention_window(q, k, v, window: int, sinks: int = 0, sm_scale: float | Non
         raise ValueError(f"flash_attn_with_score_amd: window {window} must be at least 1")
     if sinks < 0:
         raise ValueError(f"flash_attn_with_score_amd: sinks {sinks} must not be negative")
-    window, sinks = min(int(window), _MOST), min(int(sinks), _MOST)
+    window, sinks = min(operator.index(window), _MOST), min(operator.index(sinks), _MOST)
+    sm_scale = 1.0 / math.sqrt(q.shape[3]) if sm_scale is None else float(sm_scale)
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
-        _, out, L = _forward(q, k, v, window, sinks, sm_scale, return_log_normalizer)
+        *_, out, L = _forward(q, k, v, window, sinks, sm_scale, return_log_normalizer)
         return (out, L) if return_log_normalizer else out
     res = WindowAttention.apply(q, k, v, window, sinks, sm_scale, return_log_normalizer)
     _mark_leaves(res[0] if return_log_normalizer else res)
