@@ -371,12 +371,15 @@ constexpr int kNoWindow = 1 << 30;
 // Backward of the windowed attention (fas_window.hpp).  part: fp32 dK | dV of
 // parts of key blocks, slabs of 128 keys x 2D, two for each workgroup of the
 // dK/dV kernel.
+// What a key block costs the dK/dV kernel beside its row tiles, in tiles.
+constexpr int kBlockUnits = 3;
+
 struct WindowBwdParams : BwdParams {
   uint32_t o_bytes;    // extent of a head's rows of o
   int window, sinks;
   int wgs;             // workgroups of the dK/dV kernel
-  int chunk;           // row tiles of each, or 0: a whole key block each
-  int64_t head_tiles;  // row tiles of a KV head's key blocks
+  int chunk;           // units of row tiles of each, or 0: a whole key block each
+  int64_t head_units;  // units of a KV head's key blocks
 };
 
 }  // namespace fas

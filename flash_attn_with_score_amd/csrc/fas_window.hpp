@@ -16,7 +16,7 @@
 //                         ones, which is M / (window + 128) times as long.
 //                         So the row tiles of all blocks (of all heads) are one
 //                         list, block after block, and every workgroup takes
-//                         an equal run of it (p.chunk tiles): parts of a block
+//                         an equal run of it (p.chunk units): parts of a block
 //                         at its ends, whole blocks between.  Parts go to fp32
 //                         slabs, two a workgroup, that window_reduce_kernel
 //                         adds in order.  Where whole blocks are even enough
@@ -117,16 +117,24 @@ __device__ __forceinline__ void window_tiles(const WindowBwdParams& p, int kb, i
   lo = rlo / 64;
   n = max(0, (rhi + 63) / 64 - lo);
 }
-// Tiles (of G heads) of key blocks [0, kb) of a KV head, worked out 64 blocks at
-// a time; `find` instead: the block that tile `at` falls into, and the tiles
-// before it.
+// A block's share of the list in units: its row tiles (of G heads), and
+// kBlockUnits for what it costs beside them: K and V, the first tile's way, the
+// results.  (Without these a head's last workgroups, whose blocks are short and
+// so more, ended at 160 to 169 us where the others took 150: the backward of B1
+// H32/8 S4096 D128 window 1024 327 us, with three 315, with one or five 316 to 320.)
+__device__ __forceinline__ int window_units(const WindowBwdParams& p, int kb) {
+  int lo, n;
+  window_tiles(p, kb, lo, n);
+  return n > 0 ? n * p.G + kBlockUnits : 0;
+}
+// Units of key blocks [0, kb) of a KV head, worked out 64 blocks at a time;
+// `find` instead: the block that unit `at` falls into, and the units before it.
 __device__ __forceinline__ int64_t window_before(const WindowBwdParams& p, int kb) {
   const int lane = (int)threadIdx.x & 63;
   int64_t sum = 0;
   for (int k = 0; k < kb; k += 64) {
-    int lo, n = 0;
-    if (k + lane < kb) window_tiles(p, k + lane, lo, n);
-    sum += __builtin_amdgcn_readlane(wave_scan(n * p.G, [](int x, int y) { return x + y; }), 63);
+    const int n = k + lane < kb ? window_units(p, k + lane) : 0;
+    sum += __builtin_amdgcn_readlane(wave_scan(n, [](int x, int y) { return x + y; }), 63);
   }
   return sum;
 }
@@ -134,9 +142,8 @@ __device__ __forceinline__ int window_find(const WindowBwdParams& p, int64_t at,
   const int lane = (int)threadIdx.x & 63;
   before = 0;
   for (int k = 0;; k += 64) {
-    int lo, n = 0;
-    if (k + lane < p.nkb) window_tiles(p, k + lane, lo, n);
-    const int end = wave_scan(n * p.G, [](int x, int y) { return x + y; });
+    const int n = k + lane < p.nkb ? window_units(p, k + lane) : 0;
+    const int end = wave_scan(n, [](int x, int y) { return x + y; });
     const int total = __builtin_amdgcn_readlane(end, 63);
     if (at < before + total || k + 64 >= p.nkb) {
       const int i = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + end <= at));
@@ -154,7 +161,7 @@ struct WindowRun {
   int wg, bhk, kb;
   int tlo, tiles;  // the block's 64-row tiles [tlo, tlo + tiles) of every head
   int s0, s1;      // of its G * tiles, in head order
-  int64_t at, stop, before, start;  // tiles of the list: the run's, those before the block
+  int64_t at, stop, before, start;  // units of the list: the run's, those before the block
                                     // in its KV head, and the block's first
   // The run's first block (false: no tiles left for this workgroup).  Runs that
   // follow each other go to one XCD (workgroup i runs on XCD i % 8): they share
@@ -165,10 +172,10 @@ struct WindowRun {
     if (p.chunk > 0) {
       wg = (wg & 7) * ((int)gridDim.x >> 3) + (wg >> 3);
       at = (int64_t)wg * p.chunk;
-      stop = min(at + p.chunk, (int64_t)p.B * p.Hk * p.head_tiles);
+      stop = min(at + p.chunk, (int64_t)p.B * p.Hk * p.head_units);
       if (at >= stop) return false;
-      bhk = (int)(at / p.head_tiles);
-      kb = window_find(p, at - (int64_t)bhk * p.head_tiles, before);
+      bhk = (int)(at / p.head_units);
+      kb = window_find(p, at - (int64_t)bhk * p.head_units, before);
     } else {
       kb = wg / (p.B * p.Hk);  // longest first: blocks with sinks
       bhk = wg - kb * (p.B * p.Hk);
@@ -182,20 +189,22 @@ struct WindowRun {
     window_tiles(p, kb, tlo, tiles);
     s0 = 0;
     s1 = p.G * tiles;
-    start = (int64_t)bhk * p.head_tiles + before;
+    start = (int64_t)bhk * p.head_units + before;
     if (p.chunk > 0) {
-      s0 = __builtin_amdgcn_readfirstlane((int)(at - start));
-      s1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)s1, stop - start));
+      s0 = __builtin_amdgcn_readfirstlane((int)max((int64_t)0, at - start - kBlockUnits));
+      s1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)s1, stop - start - kBlockUnits));
     }
   }
   __device__ __forceinline__ bool whole(const WindowBwdParams& p) const {
     return s0 == 0 && s1 == p.G * tiles;
   }
-  // The next block with rows (blocks that no row sees take no tiles).
+  // The next block with rows (blocks that no row sees take no units), if the
+  // run reaches its tiles.
   __device__ __forceinline__ bool next(const WindowBwdParams& p) {
-    if (p.chunk == 0 || start + s1 >= stop) return false;
-    at = start + s1;
-    before += p.G * tiles;
+    const int units = p.G * tiles + kBlockUnits;
+    at = start + units;
+    if (p.chunk == 0 || at + kBlockUnits >= stop) return false;
+    before += units;
     do {
       if (++kb == p.nkb) {
         kb = 0;
@@ -207,9 +216,9 @@ struct WindowRun {
     set(p);
     return true;
   }
-  // Slab of this workgroup's part: 2 wg where it starts the run, else 2 wg + 1.
+  // Slab of this workgroup's part: 2 wg of its run's first block, else 2 wg + 1.
   __device__ __forceinline__ int slab(const WindowBwdParams& p) const {
-    return 2 * wg + (start + s0 == (int64_t)wg * p.chunk ? 0 : 1);
+    return 2 * wg + (start > (int64_t)wg * p.chunk ? 1 : 0);
   }
 };
 
@@ -517,18 +526,21 @@ __device__ __forceinline__ void window_dkdv(const WindowBwdParams& p, WindowDkdv
     f32x16 acc[DB];  // dV^T or dK^T
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
-    // Tile `t` of head h0 + hh on its way to stage st; its row values into a
-    // register of the waves' first (nl) and fifth (-delta).
-    float rv = 0.f;
-    auto fetch = [&](int hh, int t, int st) __attribute__((always_inline)) {
+    // The head whose tiles are fetched: its rows of Q or dO, and of nl or -delta.
+    i32x4 rsrc;
+    const float* rowv;
+    auto head = [&](int hh) __attribute__((always_inline)) {
       const int h = h0 + hh;
-      const i32x4 r = first ? make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes)
-                            : make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
-      dma.fetch(r, t * TQ, 0, 0, dma_base + (uint32_t)(st * TILE * 2));
-      if (kw == 0) {
-        const int64_t row = ((int64_t)b * p.H + h) * p.Mpad + t * TQ + lane;
-        rv = first ? p.nl[row] : p.delta[row];
-      }
+      rsrc = first ? make_rsrc_words(p.q + b * p.sq0 + h * p.sq1, p.q_bytes)
+                   : make_rsrc_words(p.dout + b * p.sg0 + h * p.sg1, p.g_bytes);
+      rowv = (first ? p.nl : p.delta) + ((int64_t)b * p.H + h) * p.Mpad + lane;
+    };
+    // Its tile `t` on its way to stage st; the row values into a register of the
+    // waves' first (nl) and fifth (-delta).
+    float rv = 0.f;
+    auto fetch = [&](int t, int st) __attribute__((always_inline)) {
+      dma.fetch(rsrc, t * TQ, 0, 0, dma_base + (uint32_t)(st * TILE * 2));
+      if (kw == 0) rv = rowv[t * TQ];
     };
     auto land = [&](int st) __attribute__((always_inline)) {
       vm_wait_all();
@@ -632,8 +644,9 @@ __device__ __forceinline__ void window_dkdv(const WindowBwdParams& p, WindowDkdv
     const int n = run.s1 - run.s0;
     int hh = n > 0 ? run.s0 / run.tiles : 0, tt = run.s0 - hh * run.tiles;  // the tile to fetch next
     int t_prev = 0, t_cur = run.tlo + tt, t_next;
+    head(hh);
     if (n > 0) {
-      fetch(hh, run.tlo + tt, 0);
+      fetch(run.tlo + tt, 0);
       land(0);
     }
     lds_barrier();
@@ -641,11 +654,11 @@ __device__ __forceinline__ void window_dkdv(const WindowBwdParams& p, WindowDkdv
     for (int i = 0; i <= n && n > 0; ++i) {
       if (++tt == run.tiles) {
         tt = 0;
-        ++hh;
+        head(++hh);
       }
       t_next = run.tlo + tt;
       const bool more = i + 1 < n;
-      if (more) fetch(hh, t_next, st_next);
+      if (more) fetch(t_next, st_next);
       if constexpr (first) {
         if (i < n) weights(st_cur, i & 1, t_cur);
       } else {
@@ -682,19 +695,18 @@ __global__ __launch_bounds__(256) void window_reduce_kernel(const WindowBwdParam
   constexpr int CPR = D / 8, KEYS = 256 / CPR, PER = kBwdBlock / KEYS;
   const int sub = (int)(blockIdx.x % PER), item = (int)(blockIdx.x / PER);
   const int bhk = item / p.nkb, kb = item - bhk * p.nkb;
-  int lo, tiles;
-  window_tiles(p, kb, lo, tiles);
-  const int64_t start = (int64_t)bhk * p.head_tiles + window_before(p, kb);
-  const int64_t w0 = start / p.chunk, w1 = tiles ? (start + (int64_t)p.G * tiles - 1) / p.chunk : w0;
-  if (tiles > 0 && w0 == w1) return;  // written by its only workgroup
+  const int units = window_units(p, kb);
+  const int64_t start = (int64_t)bhk * p.head_units + window_before(p, kb);
+  const int64_t w0 = (start + kBlockUnits) / p.chunk, w1 = (start + units - 1) / p.chunk;
+  if (units > 0 && w0 == w1) return;  // written by its only workgroup
   const int row = sub * KEYS + (int)threadIdx.x / CPR, d0 = 8 * ((int)threadIdx.x % CPR);
   const int key = kb * kBwdBlock + row;
   if (key >= p.N) return;
   float a[8] = {}, v[8] = {};
-  if (tiles > 0) {
+  if (units > 0) {
 #pragma unroll 4
     for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slab = 2 * w + (w == w0 && start != w * p.chunk ? 1 : 0);
+      const int64_t slab = 2 * w + (start > w * p.chunk ? 1 : 0);
       const float* src = p.part + (slab * kBwdBlock + row) * (2 * D) + d0;
       const f32x4 a0 = *reinterpret_cast<const f32x4*>(src);
       const f32x4 a1 = *reinterpret_cast<const f32x4*>(src + 4);

@@ -47,11 +47,11 @@ fas::RowsSplit fwd_split(const Problem& pr, int64_t window, int64_t sinks) {
 
 // How the dK/dV kernel's row tiles (64 rows, G heads) are dealt, and its
 // workspace.  One workgroup a CU runs at D = 128, two below.  Whole key blocks
-// end with the longest, or with whole rounds; equal runs of the list of tiles
-// cost about four tiles a workgroup (K and V again, and parts written) and 8 us
+// end with the longest, or with whole rounds; equal runs of the list of units
+// cost about four more a workgroup (K and V again, and parts written) and 8 us
 // for the parts' sum.  The cheaper end is taken.
 struct BwdPlan {
-  int64_t mpad, nkb, wgs, chunk, head_tiles;
+  int64_t mpad, nkb, wgs, chunk, head_units;
   size_t delta, part, total;
 };
 BwdPlan bwd_plan(const Problem& pr, int64_t window, int64_t sinks) {
@@ -65,10 +65,11 @@ BwdPlan bwd_plan(const Problem& pr, int64_t window, int64_t sinks) {
     const int64_t lo = std::max<int64_t>(0, k0 - off) / 64;
     const int64_t hi = k0 < sinks ? pr.M : std::min<int64_t>(pr.M, k0 + bk - 1 - off + std::min<int64_t>(window, pr.N));
     const int64_t n = pr.G * std::max<int64_t>(0, (hi + 63) / 64 - lo);
-    longest = std::max(longest, n);
-    w.head_tiles += n;
+    const int64_t units = n > 0 ? n + fas::kBlockUnits : 0;
+    longest = std::max(longest, units);
+    w.head_units += units;
   }
-  const int64_t all = heads * w.head_tiles, slots = pr.D == 128 ? kCus : 2 * kCus;
+  const int64_t all = heads * w.head_units, slots = pr.D == 128 ? kCus : 2 * kCus;
   const int64_t blocks = heads * w.nkb;
   w.wgs = blocks;
   if (all > 0) {
@@ -76,7 +77,7 @@ BwdPlan bwd_plan(const Problem& pr, int64_t window, int64_t sinks) {
     const double whole = std::max({(double)longest, (double)all / (double)slots,
                                    blocks <= slots ? 0.0
                                                    : mean * (double)((blocks + slots - 1) / slots)});
-    const int64_t chunk = std::max<int64_t>(4, (all + slots - 1) / slots);
+    const int64_t chunk = std::max<int64_t>(4 + fas::kBlockUnits, (all + slots - 1) / slots);
     if ((double)chunk + 4.0 + 8.0 / us_per_tile < whole && chunk < INT_MAX) {
       w.chunk = chunk;
       w.wgs = (all + chunk - 1) / chunk;
@@ -215,7 +216,7 @@ int fas_attention_window_backward(const fas_attn_args* a, int64_t window, int64_
   p.nrb = (int)(w.mpad / fas::kBwdBlock);
   p.wgs = (int)w.wgs;
   p.chunk = (int)w.chunk;
-  p.head_tiles = w.head_tiles;
+  p.head_units = w.head_units;
   p.window = (int)std::min<int64_t>(window, fas::kNoWindow);
   p.sinks = (int)std::min<int64_t>(sinks, fas::kNoWindow);
   p.sm_scale = std::fabs(pr.sm_scale);
