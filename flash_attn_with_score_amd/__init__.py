@@ -4,7 +4,9 @@ Drop-in replacements for the Python entry points of the reference's package
 (__init__.py:6-39): each returns (output, side product) from one call into a
 hand-written HIP kernel through the C ABI in include/fas.h.  `attention`
 (flash.py) adds the FlashAttention-2 backward pass; `total.total_attention`
-mirrors the reference's total.py.
+mirrors the reference's total.py.  `window.attention_window` (sliding windows
+with sinks) and `kv_cache` (a quantised KV cache and the attention over it)
+have no counterpart there.
 """
 from .attention_with_scores import attention_with_scores
 from .flash import attention

@@ -49,6 +49,17 @@ def _mark_leaves(out) -> None:
             node.metadata.setdefault(_STREAM, stream)
 
 
+def _mark_strangers(*inputs) -> None:
+    """Before a captured forward: leaves whose accumulation nodes other operators'
+    graphs hold, on a stream that cannot be asked for, get no stream at all.  (A
+    node that nothing holds goes, with its mark, when the reference here does.)"""
+    for x in inputs:
+        if x.requires_grad and x.is_leaf:
+            node = torch.autograd.graph.get_gradient_edge(x).node
+            node.metadata.setdefault(_STREAM, None)
+            del node
+
+
 def _check_capture(ctx, device) -> None:
     if not torch.cuda.is_current_stream_capturing():
         return
@@ -125,6 +136,8 @@ def attention_window(q, k, v, window: int, sinks: int = 0, sm_scale: float | Non
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         *_, out, L = _forward(q, k, v, window, sinks, sm_scale, return_log_normalizer)
         return (out, L) if return_log_normalizer else out
+    if torch.cuda.is_current_stream_capturing():
+        _mark_strangers(q, k, v)
     res = WindowAttention.apply(q, k, v, window, sinks, sm_scale, return_log_normalizer)
     _mark_leaves(res[0] if return_log_normalizer else res)
     return res

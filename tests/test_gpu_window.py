@@ -203,6 +203,34 @@ def test_captured_training_step(gpu):
     del graph
 
 
+@pytest.mark.parametrize("other", [lambda x: fas.attention(x, x, x, causal=True), lambda x: x * 2])
+def test_capture_beside_another_operators_graph_is_refused(other, gpu):
+    print("[case] captured window step beside another operator's graph", flush=True)
+    q, k, v = (t.to(gpu).requires_grad_(True)
+               for t in inputs.make_qkv(1, 2, 2, 130, 130, 32, dtype=BF16, seed=1))
+    alive = other(k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(graph):
+            out = attention_window(q, k, v, 50, 1)
+            torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    out = alive = None
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(attention_window(q, k, v, 50, 1), (q, k, v), torch.ones_like(q))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attention_window(q, k, v, 50, 1)
+        first = torch.autograd.grad(out, (q, k, v), torch.ones_like(out), retain_graph=True)
+        again = attention_window(k, q, v, 50, 1)  # (leaves of this capture's own graph)
+        torch.autograd.grad(again, (q, k, v), torch.ones_like(out))
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(first, want))
+    del graph
+
+
 def test_capture_beside_an_eager_graph_is_refused(gpu):
     """A captured backward pass while an eager graph of the same leaves lives would
     end the process in the autograd engine: it raises, and the step can be
