@@ -629,6 +629,7 @@ void few_kernel(const RowsParams p) {
 // values(stage) are its swizzled tiles; nan_blocks(stage, lane) says which of
 // tile row `lane`'s V blocks read as NaN (kNanBlocks sources: those blocks are
 // staged as zeros).
+constexpr uint32_t kMi355Cus = 256;
 template <class E, int D, class SRC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void rows_kernel(const RowsParams p) {
@@ -720,7 +721,17 @@ void rows_kernel(const RowsParams p) {
     if (t + 1 < t1) src.land(stage ^ 1);
     lds_barrier();
   };
+  // Two workgroups share a CU and the older one's waves go first: where the grid is
+  // one round, it ended after 110 us and the younger one, alone then, after 140 (B2
+  // H32/8 M512 N8000 D128 4 bits, in two parts).  So the younger one goes first for
+  // half its tiles: the call 157.8 us, so 153; B4 M256 N4000 D64 57.8, 55.0.  (In
+  // grids of several rounds the next workgroups even it out: B1 H32/8 S8192 window
+  // 256 62 us, with this 70.)
+  const bool younger = gridDim.x <= 2 * kMi355Cus && blockIdx.x >= kMi355Cus;
+  const int half = younger ? t0 + (t1 - t0) / 2 : t1;
+  if (younger) __builtin_amdgcn_s_setprio(1);
   for (int t = t0; t < t1; t += 2) {
+    if (t >= half) __builtin_amdgcn_s_setprio(0);
     step(t, std::integral_constant<int, 0>{});
     if (t + 1 < t1) step(t + 1, std::integral_constant<int, 1>{});
   }
